@@ -306,6 +306,10 @@ int silvann_b200_counters_read(uint64_t* out, uint32_t n, int reset);
  * array, because it may not allocate one — is ORed into the same answer.  clear != 0 zeroes both words. */
 #define SILVANN_B200_STATUS_TIMEOUT  0x4232544Fu
 #define SILVANN_B200_STATUS_BAD_PAGE 0x80000000u
+/* silvann_b200_paged_tables changed nothing: the free pages do not cover the step (NO_PAGES), or a length, a count, a
+ * page-table row or the row arrays do not fit it (BAD_STEP). */
+#define SILVANN_B200_STATUS_NO_PAGES 0x20000000u
+#define SILVANN_B200_STATUS_BAD_STEP 0x10000000u
 int silvann_b200_device_status(uint32_t* word, int clear);
 
 /* Fused split-KV decode of one query position over a contiguous cache — the work of attention_scores +
@@ -374,6 +378,70 @@ int silvann_b200_paged_decode(silvann_b200_plan* plan, void* o, float* res, cons
 int silvann_b200_paged_append(silvann_b200_plan* plan, void* k_pool, void* v_pool, const void* k_rows, const void* v_rows,
                               uint64_t pool_pages, uint32_t page_positions, const int32_t* page_table, uint32_t table_stride,
                               void* stream);
+
+/* ---- a serving step over the paged pool with nothing on the host: the step's tables, the rows' way into the pool, and
+ * attention over selected blocks.  Lengths, counts, tables and slots are DEVICE arrays of int32; nothing is allocated or
+ * waited for, no call keeps anything for the next and calls on different streams share no scratch, so each may be captured
+ * into a graph and replayed (after the library's first call on the device, which allocates the device's status word).
+ * Three entry points, called in this order once a step (the last two once a layer): */
+
+/* The step's tables, on the card, from the sequences' lengths.  lens[s] positions are held; counts[s] >= 0 positions come
+ * in, or SILVANN_B200_PAGED_ENDED (-1): the sequence has ended and its pages come back.  free_pages [free_total] is a stack
+ * of page numbers whose entries from *free_at on are free.  In this order: the pages of ended sequences (by sequence, then
+ * by column) go to free_pages[*free_at - R ..) where R is how many there are; then every sequence in order takes the pages
+ * it lacks for its new length, ceil(len / page_positions) of each, from free_pages[*free_at - R ..) upwards, into
+ * page_table[s][...] (columns past a sequence's last page keep what they hold, an ended sequence's row included).
+ * new_lens[s] = len + count, 0 for an ended one; *free_out = what *free_at has become.  row_start [seqs + 1]: the new
+ * positions counted up to each sequence; and for each new position, by sequence and ascending, row_seq (its sequence),
+ * row_pos (its position) and row_slot (page * page_positions + position % page_positions, its place in the pool), -1 in
+ * all three from row_start[seqs] up to `rows`.  An entry of the table or the stack that names no page of the pool gives the slot -1 and
+ * raises SILVANN_B200_STATUS_BAD_PAGE.
+ * A step that does not fit is refused on the card as a whole: when a length is negative, a count is below -1, a new length
+ * exceeds table_stride * page_positions, the new positions exceed `rows`, or *free_at is no index of the stack or below R,
+ * SILVANN_B200_STATUS_BAD_STEP is raised; when free pages are too few, SILVANN_B200_STATUS_NO_PAGES.  Then the table and the
+ * stack stay as they were, new_lens = lens, *free_out = *free_at, row_start is 0 and every row -1.
+ * new_lens may be lens and free_out may be free_at; no other two arrays may overlap.  seqs <= SILVANN_B200_PAGED_SEQS_MAX;
+ * pool_pages * page_positions <= 2^31 - 1.  A page must not be held by two sequences when one of them ends. */
+#define SILVANN_B200_PAGED_ENDED (-1)
+#define SILVANN_B200_PAGED_SEQS_MAX 8192u
+int silvann_b200_paged_tables(int32_t* new_lens, int32_t* page_table, int32_t* row_start, int32_t* row_seq, int32_t* row_pos,
+                              int32_t* row_slot, uint32_t* free_out, int32_t* free_pages, const uint32_t* free_at,
+                              const int32_t* lens, const int32_t* counts, uint32_t seqs, uint32_t table_stride, uint32_t rows,
+                              uint32_t free_total, uint64_t pool_pages, uint32_t page_positions, void* stream);
+
+/* Writes rows into the pools (paged_decode's) by slot: k_pool[row_slot[r]] = k_rows[r], the same for v, [kv_heads][head_dim]
+ * 16-bit elements a row; a negative slot is padding and is skipped; a slot past the pool is skipped and raises
+ * SILVANN_B200_STATUS_BAD_PAGE.  k_stride and v_stride are the elements from one row to the next (0: packed), so that rows
+ * may be read out of a wider projection.  With block_positions B (16, 32, 64 or 128, a divisor of page_positions; 0: k_means
+ * is not touched) a row that is the last of a block, slot % B == B - 1, also leaves the block's mean key at
+ * k_means[slot / B][kv_heads][head_dim]: the fp32 sum of the block's B rows in ascending order, over B, rounded to `dtype`.
+ * Rows of one block must stand in ascending order next to each other (as paged_tables numbers them), earlier ones in the
+ * pool; no slot may be named twice.  kv_heads * head_dim and the strides are multiples of 8, addresses of 16 bytes. */
+int silvann_b200_paged_write(void* k_pool, void* v_pool, void* k_means, const void* k_rows, const void* v_rows, uint64_t k_stride,
+                             uint64_t v_stride, const int32_t* row_slot, uint32_t rows, uint32_t kv_heads, uint32_t head_dim,
+                             uint64_t pool_pages, uint32_t page_positions, uint32_t block_positions, int dtype, void* stream);
+
+/* Attention of `rows` new positions over selected blocks of their sequences.  Row r is position p = row_pos[r] of sequence
+ * row_seq[r] < seqs, whose n = p / B + 1 blocks of B = block_positions it may attend.  A row attends at most first + last + top
+ * of them: all n when they are no more; else, for every kv head, the first `first`, the last `last` (at least 1: the row's
+ * own block) and of those between the `top` with the greatest score, the dot product of the sum of the kv head's query heads
+ * with the block's mean key.  The score is taken in 64 bits, a NaN ranks as minus infinity, equal scores go to the lower
+ * block: the choice does not depend on how the work is split.  Within the chosen blocks it is ordinary causal attention,
+ * scale 1 / sqrt(head_dim).
+ * q [rows][q_heads][head_dim], q_stride elements from row to row (0: packed); o [rows][q_heads][head_dim] and/or res
+ * [rows][q_heads][head_dim + 2] fp32 (m, l, acc); chosen (may be null) [rows][kv_heads][first + last + top] the blocks'
+ * numbers, ascending, -1 behind the last.  Pools, page_table [seqs][table_stride] and bad pages as paged_decode; a bad page's
+ * blocks score minus infinity.  k_means as paged_write leaves it; it may be null when top is 0.  A row whose row_seq is
+ * negative is padding: its outputs stay as they were; one with row_seq >= seqs is treated the same and raises
+ * SILVANN_B200_STATUS_BAD_PAGE.  A row at a negative position attends nothing: o is 0, res (-inf, 0, 0), chosen -1.
+ * head_dim 64, 128 or 256; up to 64 query heads a kv head; B 16, 32, 64 or 128 and a divisor of page_positions;
+ * first + last + top <= SILVANN_B200_PAGED_KEEP_MAX; rows of q multiples of 8 elements, addresses of 16 bytes. */
+#define SILVANN_B200_PAGED_KEEP_MAX 1024u
+int silvann_b200_paged_sparse(void* o, float* res, int32_t* chosen, const void* q, uint64_t q_stride, const void* k_pool, const void* v_pool,
+                              const void* k_means, const int32_t* row_seq, const int32_t* row_pos, uint32_t rows, const int32_t* page_table,
+                              uint32_t seqs, uint32_t table_stride, uint64_t pool_pages, uint32_t page_positions, uint32_t block_positions,
+                              uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t first, uint32_t last, uint32_t top, int dtype,
+                              sv_fault* over, void* stream);
 
 /* One query position over a two-tier cache: the oldest host_len positions in pinned host RAM (k_host, v_host are HOST
  * addresses of [host_len][kv_heads][head_dim] planes), the next dev_len positions on the card.  The reference has no

@@ -17,6 +17,8 @@
 #define SV_FAULT_OVERFLOW 0x4E504F56u   /* "NPOV" — engine/src/packages/nn/contracts/objects/primitives.cuh:57 */
 #define SV_STATUS_TIMEOUT 0x4232544Fu   /* "B2TO" — a bounded device-side wait gave up */
 #define SV_STATUS_BAD_PAGE 0x80000000u  /* a page-table entry inside a sequence's length named no page of the pool (a bit the code above leaves clear) */
+#define SV_STATUS_NO_PAGES 0x20000000u  /* a step's tables were refused: too few free pages */
+#define SV_STATUS_BAD_STEP 0x10000000u  /* a step's tables were refused: a length, a count, a table row or the row arrays do not fit */
 
 /* How long a device-side wait may spin before giving up: tries of mbarrier.try_wait (each suspends for a
  * hardware-chosen slice) — in the order of a second at worst, far beyond any healthy TMA or MMA latency. */

@@ -1,0 +1,258 @@
+/* paged.cu — a serving step's tables built on the card, and the rows' way into the paged pool with the blocks' mean keys
+ * (declared in include/silvann_b200.h). */
+#include "../../include/silvann_b200.h"
+#include "common.cuh"
+#include "kernels.h"
+#include "paged_index.h"
+#include <atomic>
+#include <string.h>
+
+#define SV_EXPORT extern "C" __attribute__((visibility("default")))
+
+int sv_ext_fail(int code, const char* fmt, ...);      /* ext.cu: records the message for silvann_b200_last_error */
+namespace svf { extern std::atomic<uint64_t> g_counters[SILVANN_B200_COUNTERS]; }
+static inline void called() { svf::g_counters[SILVANN_B200_COUNTER_EXT_CALLS].fetch_add(1, std::memory_order_relaxed); }
+
+namespace sv {
+
+/* ---------------------------------------------------------------------------------------------------------- */
+/* the step's tables                                                                                            */
+
+#define SV_TABLES_THREADS 1024
+static constexpr int TABLES_DEVICES = 64;
+
+struct TablesParams {
+    int32_t *new_lens, *table, *row_start, *row_seq, *row_pos, *row_slot;
+    uint32_t* free_out;
+    int32_t* free_pages;
+    const uint32_t* free_at;
+    const int32_t *lens, *counts;
+    unsigned int* status;
+    uint32_t seqs, stride, rows, free_total, pool_pages, page_pos;
+};
+
+/* What one sequence brings to the three sums: new positions, pages it takes, pages it gives back. */
+struct TablesItem { uint32_t rows, need, back; bool bad; };
+__device__ __forceinline__ TablesItem tables_item(const TablesParams& P, int32_t len, int32_t count) {
+    TablesItem it = {0u, 0u, 0u, false};
+    const uint64_t most = (uint64_t)P.stride * P.page_pos;
+    if (len < 0 || count < SILVANN_B200_PAGED_ENDED || (uint64_t)len + (uint64_t)(count > 0 ? count : 0) > most ||
+        (int64_t)len + (count > 0 ? count : 0) > 0x7FFFFFFFll) { it.bad = true; return it; }
+    const uint32_t held = ((uint32_t)len + P.page_pos - 1u) / P.page_pos;
+    if (count < 0) it.back = held;
+    else { it.rows = (uint32_t)count; it.need = ((uint32_t)len + (uint32_t)count + P.page_pos - 1u) / P.page_pos - held; }
+    return it;
+}
+
+/* The sequence that item j of a list belongs to: the last s with start[s] <= j among those that have items. */
+__device__ __forceinline__ uint32_t tables_owner(const uint32_t* start, uint32_t seqs, uint32_t j) {
+    uint32_t lo = 0u, hi = seqs;                       /* start[lo] <= j < start[hi] */
+    while (hi - lo > 1u) { const uint32_t mid = (lo + hi) >> 1; if (start[mid] <= j) lo = mid; else hi = mid; }
+    return lo;
+}
+
+/* Exclusive sums of (rows, need, back) over the sequences, then three flat lists — pages that come back, pages handed out,
+ * new positions — walked by all threads.  The whole step is decided (fits or is refused) before anything is written. */
+__global__ void __launch_bounds__(SV_TABLES_THREADS, 1) paged_tables_kernel(const TablesParams P) {
+    extern __shared__ uint32_t tsm[];
+    uint32_t* rows_s = tsm;                       /* [seqs + 1] each */
+    uint32_t* need_s = rows_s + P.seqs + 1;
+    uint32_t* back_s = need_s + P.seqs + 1;
+    int32_t* len_s = (int32_t*)(back_s + P.seqs + 1);
+    __shared__ unsigned long long warp_sum[3][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t per = (P.seqs + SV_TABLES_THREADS - 1) / SV_TABLES_THREADS;
+    const uint32_t i0 = min(P.seqs, tid * per), i1 = min(P.seqs, i0 + per);
+    const uint32_t at = *P.free_at;
+
+    unsigned long long sum[3] = {0, 0, 0};
+    bool bad = false;
+    for (uint32_t s = i0; s < i1; ++s) {
+        const TablesItem it = tables_item(P, P.lens[s], P.counts[s]);
+        sum[0] += it.rows; sum[1] += it.need; sum[2] += it.back; bad |= it.bad;
+    }
+    unsigned long long before[3];
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+        unsigned long long v = sum[x];
+        for (int d = 1; d < 32; d <<= 1) { const unsigned long long o = __shfl_up_sync(0xffffffffu, v, d); if (lane >= d) v += o; }
+        if (lane == 31) warp_sum[x][warp] = v;
+        before[x] = v - sum[x];
+    }
+    bad = __syncthreads_or(bad);
+    unsigned long long all[3];
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+        unsigned long long w = 0, mine = 0;
+        for (int u = 0; u < 32; ++u) { if (u == warp) mine = w; w += warp_sum[x][u]; }
+        before[x] += mine; all[x] = w;
+    }
+    const bool bad_step = bad || all[0] > P.rows || at > P.free_total || all[2] > at;
+    const bool no_pages = !bad_step && all[1] > (unsigned long long)P.free_total - (at - all[2]);
+
+    if (bad_step || no_pages) {
+        if (tid == 0) {
+            if (P.status) atomicOr(P.status, bad_step ? SV_STATUS_BAD_STEP : SV_STATUS_NO_PAGES);
+            *P.free_out = at;
+        }
+        for (uint32_t s = tid; s <= P.seqs; s += blockDim.x) { if (s < P.seqs) P.new_lens[s] = P.lens[s]; P.row_start[s] = 0; }
+        for (uint32_t r = tid; r < P.rows; r += blockDim.x) { P.row_seq[r] = -1; P.row_pos[r] = -1; P.row_slot[r] = -1; }
+        return;
+    }
+    for (uint32_t s = i0; s < i1; ++s) {
+        const int32_t len = P.lens[s];
+        const TablesItem it = tables_item(P, len, P.counts[s]);
+        rows_s[s] = (uint32_t)before[0]; need_s[s] = (uint32_t)before[1]; back_s[s] = (uint32_t)before[2]; len_s[s] = len;
+        before[0] += it.rows; before[1] += it.need; before[2] += it.back;
+    }
+    if (tid == 0) { rows_s[P.seqs] = (uint32_t)all[0]; need_s[P.seqs] = (uint32_t)all[1]; back_s[P.seqs] = (uint32_t)all[2]; }
+    __syncthreads();
+    const uint32_t n_rows = (uint32_t)all[0], n_need = (uint32_t)all[1], n_back = (uint32_t)all[2], bottom = at - n_back;
+    bool strange = false;                          /* an entry that names no page of the pool */
+
+    for (uint32_t j = tid; j < n_back; j += blockDim.x) {
+        const uint32_t s = tables_owner(back_s, P.seqs, j);
+        const int32_t page = P.table[(size_t)s * P.stride + (j - back_s[s])];
+        strange |= page < 0 || (uint32_t)page >= P.pool_pages;
+        P.free_pages[bottom + j] = page;
+    }
+    __syncthreads();
+    for (uint32_t s = tid; s <= P.seqs; s += blockDim.x) {
+        P.row_start[s] = (int32_t)rows_s[s];
+        if (s < P.seqs) P.new_lens[s] = back_s[s + 1] > back_s[s] ? 0 : len_s[s] + (int32_t)(rows_s[s + 1] - rows_s[s]);
+    }
+    if (tid == 0) *P.free_out = bottom + n_need;
+    for (uint32_t j = tid; j < n_need; j += blockDim.x) {
+        const uint32_t s = tables_owner(need_s, P.seqs, j);
+        const int32_t page = P.free_pages[bottom + j];
+        strange |= page < 0 || (uint32_t)page >= P.pool_pages;
+        P.table[(size_t)s * P.stride + ((uint32_t)len_s[s] + P.page_pos - 1u) / P.page_pos + (j - need_s[s])] = page;
+    }
+    for (uint32_t r = tid; r < P.rows; r += blockDim.x) {
+        int32_t seq = -1, pos = -1, slot = -1;
+        if (r < n_rows) {
+            const uint32_t s = tables_owner(rows_s, P.seqs, r);
+            const uint32_t len = (uint32_t)len_s[s], p = len + (r - rows_s[s]), col = p / P.page_pos, held = (len + P.page_pos - 1u) / P.page_pos;
+            /* a page taken in this step is read from the stack, where it came from */
+            const int32_t page = col < held ? P.table[(size_t)s * P.stride + col] : P.free_pages[bottom + need_s[s] + (col - held)];
+            seq = (int32_t)s; pos = (int32_t)p;
+            if (page < 0 || (uint32_t)page >= P.pool_pages) strange = true;
+            else slot = (int32_t)((uint32_t)page * P.page_pos + (p - col * P.page_pos));
+        }
+        P.row_seq[r] = seq; P.row_pos[r] = pos; P.row_slot[r] = slot;
+    }
+    if (strange && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE);
+}
+
+static cudaError_t tables_launch(const TablesParams& P, cudaStream_t st) {
+    const size_t smem = (size_t)4 * (P.seqs + 1) * sizeof(uint32_t);
+    static std::atomic<bool> attr_set[TABLES_DEVICES];
+    int d = 0; cudaGetDevice(&d);
+    if (d >= 0 && d < TABLES_DEVICES && !attr_set[d].load(std::memory_order_acquire)) {
+        cudaError_t e = cudaFuncSetAttribute(paged_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((size_t)4 * (SILVANN_B200_PAGED_SEQS_MAX + 1) * sizeof(uint32_t)));
+        if (e != cudaSuccess) return e;
+        attr_set[d].store(true, std::memory_order_release);
+    }
+    paged_tables_kernel<<<1, SV_TABLES_THREADS, smem, st>>>(P);
+    note_launch(1);
+    return cudaGetLastError();
+}
+
+/* ---------------------------------------------------------------------------------------------------------- */
+/* rows into the pool                                                                                           */
+
+struct WriteParams {
+    uint4 *k_pool, *v_pool, *means;
+    const uint4 *k_rows, *v_rows;
+    const int32_t* slots;
+    unsigned int* status;
+    uint64_t k_stride, v_stride;        /* in uint4 */
+    uint32_t rows, row_vec, pool_slots, block;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(128) paged_write_kernel(const WriteParams P) {
+    using E = Elem<DT>;
+    const uint32_t r = blockIdx.x;
+    const int32_t slot = P.slots[r];
+    if (slot < 0) return;
+    if ((uint32_t)slot >= P.pool_slots) { if (threadIdx.x == 0 && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE); return; }
+    const bool whole = P.block && (uint32_t)slot % P.block == P.block - 1u;
+    for (uint32_t i = threadIdx.x; i < P.row_vec; i += blockDim.x) {
+        P.k_pool[(size_t)slot * P.row_vec + i] = P.k_rows[r * P.k_stride + i];
+        P.v_pool[(size_t)slot * P.row_vec + i] = P.v_rows[r * P.v_stride + i];
+        if (!whole) continue;
+        /* the block's other rows: as far back as this call's rows run on, from the call, before that from the pool */
+        uint32_t here = 1;
+        while (here < P.block && here <= r && P.slots[r - here] == slot - (int32_t)here) ++here;
+        float sum[8] = {};
+        for (uint32_t b = 0; b < P.block; ++b) {
+            const uint32_t back = P.block - 1u - b;
+            const uint4 x = back < here ? P.k_rows[(uint64_t)(r - back) * P.k_stride + i] : P.k_pool[(size_t)(slot - back) * P.row_vec + i];
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { const float2 f = E::unpack2(w[u]); sum[2 * u] += f.x; sum[2 * u + 1] += f.y; }
+        }
+        const float inv = 1.0f / (float)P.block;
+        uint4 m;
+        m.x = E::pack2(sum[0] * inv, sum[1] * inv); m.y = E::pack2(sum[2] * inv, sum[3] * inv);
+        m.z = E::pack2(sum[4] * inv, sum[5] * inv); m.w = E::pack2(sum[6] * inv, sum[7] * inv);
+        P.means[(size_t)((uint32_t)slot / P.block) * P.row_vec + i] = m;
+    }
+}
+
+}  // namespace sv
+
+static inline bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+static int cuda_fail(const char* what, cudaError_t e) {
+    (void)cudaGetLastError();
+    return sv_ext_fail(SILVANN_B200_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+SV_EXPORT int silvann_b200_paged_tables(int32_t* new_lens, int32_t* page_table, int32_t* row_start, int32_t* row_seq, int32_t* row_pos, int32_t* row_slot,
+                                        uint32_t* free_out, int32_t* free_pages, const uint32_t* free_at, const int32_t* lens, const int32_t* counts,
+                                        uint32_t seqs, uint32_t table_stride, uint32_t rows, uint32_t free_total, uint64_t pool_pages,
+                                        uint32_t page_positions, void* stream) {
+    called();
+    const void* all[] = {new_lens, page_table, row_start, row_seq, row_pos, row_slot, free_out, free_pages, free_at, lens, counts};
+    for (const void* p : all) if (!p || !aligned(p, 4)) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_tables: an operand is null or not 4-byte aligned");
+    if (seqs == 0 || seqs > SILVANN_B200_PAGED_SEQS_MAX) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_tables: %u sequences (1 to %u)", seqs, SILVANN_B200_PAGED_SEQS_MAX);
+    if (table_stride == 0 || rows == 0 || rows > 0x7FFFFFFFu || free_total == 0 || free_total > 0x7FFFFFFFu)
+        return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_tables: %u table columns, %u rows, a stack of %u pages", table_stride, rows, free_total);
+    if (pool_pages == 0 || page_positions == 0 || pool_pages > 0x7FFFFFFFull / page_positions)
+        return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_tables: pool of %llu pages of %u positions", (unsigned long long)pool_pages, page_positions);
+    sv::TablesParams P;
+    P.new_lens = new_lens; P.table = page_table; P.row_start = row_start; P.row_seq = row_seq; P.row_pos = row_pos; P.row_slot = row_slot;
+    P.free_out = free_out; P.free_pages = free_pages; P.free_at = free_at; P.lens = lens; P.counts = counts; P.status = sv::device_status_word();
+    P.seqs = seqs; P.stride = table_stride; P.rows = rows; P.free_total = free_total; P.pool_pages = (uint32_t)pool_pages; P.page_pos = page_positions;
+    cudaError_t e = sv::tables_launch(P, (cudaStream_t)stream);
+    return e == cudaSuccess ? SILVANN_B200_OK : cuda_fail("paged_tables: launch", e);
+}
+
+SV_EXPORT int silvann_b200_paged_write(void* k_pool, void* v_pool, void* k_means, const void* k_rows, const void* v_rows, uint64_t k_stride,
+                                       uint64_t v_stride, const int32_t* row_slot, uint32_t rows, uint32_t kv_heads, uint32_t head_dim,
+                                       uint64_t pool_pages, uint32_t page_positions, uint32_t block_positions, int dtype, void* stream) {
+    called();
+    if (!k_pool || !v_pool || !k_rows || !v_rows || !row_slot || (block_positions && !k_means)) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_write: a null operand");
+    if (dtype != SILVANN_B200_DTYPE_FP16 && dtype != SILVANN_B200_DTYPE_BF16) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_write: dtype %d", dtype);
+    const uint64_t row = (uint64_t)kv_heads * head_dim;
+    if (k_stride == 0) k_stride = row;
+    if (v_stride == 0) v_stride = row;
+    if (rows == 0 || rows > 0x7FFFFFFFu || row == 0 || row > (1ull << 20) || row % 8u || k_stride % 8u || v_stride % 8u || k_stride < row || v_stride < row)
+        return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_write: %u rows of %u x %u elements, %llu and %llu apart (multiples of 8)", rows, kv_heads, head_dim, (unsigned long long)k_stride, (unsigned long long)v_stride);
+    if (pool_pages == 0 || page_positions == 0 || pool_pages > 0x7FFFFFFFull / page_positions)
+        return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_write: pool of %llu pages of %u positions", (unsigned long long)pool_pages, page_positions);
+    if (block_positions && ((block_positions != 16 && block_positions != 32 && block_positions != 64 && block_positions != 128) || page_positions % block_positions))
+        return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_write: blocks of %u positions (16, 32, 64 or 128) in pages of %u", block_positions, page_positions);
+    if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(k_rows, 16) || !aligned(v_rows, 16) || !aligned(row_slot, 4) || (block_positions && !aligned(k_means, 16)))
+        return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_write: rows, pools and means must be 16-byte aligned");
+    sv::WriteParams P;
+    P.k_pool = (uint4*)k_pool; P.v_pool = (uint4*)v_pool; P.means = (uint4*)k_means; P.k_rows = (const uint4*)k_rows; P.v_rows = (const uint4*)v_rows;
+    P.slots = row_slot; P.status = sv::device_status_word(); P.k_stride = k_stride / 8u; P.v_stride = v_stride / 8u; P.rows = rows; P.row_vec = (uint32_t)(row / 8u);
+    P.pool_slots = (uint32_t)(pool_pages * page_positions); P.block = block_positions;
+    if (dtype == SILVANN_B200_DTYPE_FP16) sv::paged_write_kernel<SV_DTYPE_FP16><<<rows, 128, 0, (cudaStream_t)stream>>>(P);
+    else sv::paged_write_kernel<SV_DTYPE_BF16><<<rows, 128, 0, (cudaStream_t)stream>>>(P);
+    sv::note_launch(1);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? SILVANN_B200_OK : cuda_fail("paged_write: launch", e);
+}

@@ -21,6 +21,7 @@ EXPORTS = (
     "silvann_b200_exchange_create", "silvann_b200_exchange_destroy", "silvann_b200_exchange_local", "silvann_b200_exchange_handle",
     "silvann_b200_exchange_connect_handles", "silvann_b200_exchange_connect_addresses", "silvann_b200_exchange_merge_finish",
     "silvann_b200_exchange_vector_sum", "silvann_b200_exchange_deposit", "silvann_b200_mla_decode", "silvann_b200_exchange_gemv_sum",
+    "silvann_b200_paged_tables", "silvann_b200_paged_write", "silvann_b200_paged_sparse",
 )
 
 
@@ -60,6 +61,9 @@ def lib():
             "silvann_b200_plan_info": [vp, vp, vp, vp],
             "silvann_b200_paged_decode": [vp, vp, vp, vp, vp, vp, u64, u32, vp, u32, i32, vp, vp],
             "silvann_b200_paged_append": [vp, vp, vp, vp, vp, u64, u32, vp, u32, vp],
+            "silvann_b200_paged_tables": [vp] * 11 + [u32, u32, u32, u32, u64, u32, vp],
+            "silvann_b200_paged_write": [vp, vp, vp, vp, vp, u64, u64, vp, u32, u32, u32, u64, u32, u32, i32, vp],
+            "silvann_b200_paged_sparse": [vp, vp, vp, vp, u64, vp, vp, vp, vp, vp, u32, vp, u32, u32, u64, u32, u32, u32, u32, u32, u32, u32, u32, i32, vp, vp],
             "silvann_b200_tier_create": [vp, u32, u32, u32, i32, u32, u32],
             "silvann_b200_tier_destroy": [vp],
             "silvann_b200_tier_decode": [vp, vp, vp, vp, vp, vp, u64, vp, vp, u64, vp, vp],
@@ -166,6 +170,33 @@ class Plan:
     def append(self, k_pool, v_pool, k_rows, v_rows, pool_pages, page_positions, page_table, table_stride, stream=None):
         _check(lib().silvann_b200_paged_append(self.handle, addr(k_pool), addr(v_pool), addr(k_rows), addr(v_rows), pool_pages, page_positions,
                                                addr(page_table), table_stride, stream))
+
+
+PAGED_ENDED = -1
+PAGED_SEQS_MAX, PAGED_KEEP_MAX = 8192, 1024
+
+
+def paged_tables(new_lens, page_table, row_start, row_seq, row_pos, row_slot, free_out, free_pages, free_at, lens, counts, seqs, table_stride, rows, free_total,
+                 pool_pages, page_positions, stream=None):
+    """A step's tables on the card, from the sequences' lengths and counts (see silvann_b200_paged_tables)."""
+    _check(lib().silvann_b200_paged_tables(addr(new_lens), addr(page_table), addr(row_start), addr(row_seq), addr(row_pos), addr(row_slot), addr(free_out),
+                                           addr(free_pages), addr(free_at), addr(lens), addr(counts), seqs, table_stride, rows, free_total, pool_pages,
+                                           page_positions, stream))
+
+
+def paged_write(k_pool, v_pool, k_means, k_rows, v_rows, row_slot, rows, kv_heads, head_dim, pool_pages, page_positions, block_positions=0, k_stride=0, v_stride=0,
+                dtype=FP16, stream=None):
+    """Rows into the pools by slot, and the mean key of every block they complete (see silvann_b200_paged_write)."""
+    _check(lib().silvann_b200_paged_write(addr(k_pool), addr(v_pool), addr(k_means), addr(k_rows), addr(v_rows), k_stride, v_stride, addr(row_slot), rows, kv_heads,
+                                          head_dim, pool_pages, page_positions, block_positions, dtype, stream))
+
+
+def paged_sparse(o, res, chosen, q, k_pool, v_pool, k_means, row_seq, row_pos, rows, page_table, seqs, table_stride, pool_pages, page_positions, block_positions,
+                 q_heads, kv_heads, head_dim, first, last, top, q_stride=0, dtype=FP16, over=None, stream=None):
+    """Attention of new positions over the blocks a cheap score selects (see silvann_b200_paged_sparse)."""
+    _check(lib().silvann_b200_paged_sparse(addr(o), addr(res), addr(chosen), addr(q), q_stride, addr(k_pool), addr(v_pool), addr(k_means), addr(row_seq), addr(row_pos),
+                                           rows, addr(page_table), seqs, table_stride, pool_pages, page_positions, block_positions, q_heads, kv_heads, head_dim,
+                                           first, last, top, dtype, addr(over), stream))
 
 
 class Tier:
