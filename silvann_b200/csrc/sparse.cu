@@ -1,9 +1,27 @@
 /* sparse.cu — attention of new positions over the blocks of the paged pool that a cheap score selects
- * (silvann_b200_paged_sparse, include/silvann_b200.h). */
+ * (silvann_b200_paged_sparse, include/silvann_b200.h): scores, choice and attention in one launch.
+ *
+ * A cluster of thread blocks (1 to 16) owns one row's query heads over one kv head (16 at most: more heads are more
+ * clusters, which make the same choice).  Three phases:
+ *
+ *   scores  — every block's mean key is read once, from L2 or memory, and multiplied with the sum of the kv head's query
+ *             heads; the cluster's thread blocks share the sequence's blocks and leave every score, in 64 bits, in every
+ *             thread block's shared memory.
+ *   choice  — each thread block picks the same `top` blocks from the whole list, so nothing has to be sent round again.
+ *   attend  — the chosen blocks, in order, are a short cache of their own: 64-position tiles of it are dealt to the thread
+ *             blocks, arrive by TMA (128-byte swizzle) in a ring, and meet an online softmax with heads as the N dimension
+ *             of the warp MMAs (S^T = K Q^T, O^T = V^T P^T).  Four warps share a tile by positions, and two such sets share it
+ *             by value columns (both form the scores, which is cheaper than a second set of accumulators).  The partials
+ *             meet through the cluster's shared memory, in a fixed order.  No scratch in global memory: calls share nothing.
+ *
+ * Why 64 bits for the scores: which block is chosen hangs on two scores next to each other, and a choice that went by the
+ * order of a sum in fp32 would be one of the launch's shape.  The products of 16-bit values are exact there and the tree
+ * over a mean's columns is the same wherever the mean lies. */
 #include "../../include/silvann_b200.h"
 #include "common.cuh"
 #include "kernels.h"
 #include "paged_index.h"
+#include "tensormap.cuh"
 #include <atomic>
 #include <math.h>
 #include <string.h>
@@ -16,19 +34,56 @@ namespace svf { extern std::atomic<uint64_t> g_counters[SILVANN_B200_COUNTERS]; 
 namespace sv {
 
 static constexpr int SPARSE_DEVICES = 64;
-#define SP_THREADS 256
-#define SP_CHUNK 2048u      /* scores looked at in one go; the best of the chunks before them ride along */
+#define SP_WARPS 8                            /* warps that score, choose and multiply; one more issues the loads */
+#define SP_THREADS (SP_WARPS * 32)
+#define SP_CHUNK 4096u                        /* scores looked at in one go; the best of the chunks before them ride along */
+#define SP_BINS 256u
+#define SP_LIST 128u
+
+template <int D> struct SparseCfg {
+    static constexpr int BOXES = D / 64;                  /* 64-column (128-byte) boxes a row */
+    static constexpr int BOX_BYTES = 64 * 128;            /* 64 positions */
+    static constexpr int K_BYTES = BOXES * BOX_BYTES;
+    static constexpr int STAGE_BYTES = 2 * K_BYTES;       /* K then V */
+    static constexpr int STAGES = D == 64 ? 6 : 3;        /* 96 KB at head_dim 64 and 128 (two thread blocks an SM), 192 KB at 256 */
+    /* scores: lanes a mean, 16-byte pieces of it a lane, means a warp takes at a time */
+    static constexpr int LPB = D == 256 ? 16 : 8;
+    static constexpr int CPL = D / 8 / LPB;
+    static constexpr int BPS = 32 / LPB;
+    static constexpr int U = 4;
+    static constexpr int WB = BPS * U;
+};
 
 struct SparseParams {
     void* o;
     float* res;
     int32_t* chosen;
-    const uint16_t *q, *k, *v, *means;
+    const uint16_t *q, *means;
     const int32_t *row_seq, *row_pos, *table;
     unsigned int *over, *status;
     uint64_t q_stride;
-    uint32_t seqs, stride, pool_pages, page_pos, block, q_heads, kv_heads, group, first, last, top;
-    float scale;
+    uint32_t seqs, stride, pool_pages, page_pos, block, q_heads, kv_heads, group, head_blocks, first, last, top;
+    float scale_log2;
+};
+
+/* 16-bit values as doubles without a conversion (those run at a quarter of the multiply-adds' rate): the exponent and
+ * mantissa bits moved to their place in a double's high word, which is the value times 2^-896 (bf16) or 2^-1008 (fp16),
+ * subnormals included.  The query sum carries 2^800 or 2^900, so a score comes out times 2^-SHIFT.  An infinity or a NaN
+ * would come out finite: `special` collects the magnitudes, and a mean that has one is summed again by conversion. */
+template <int DT> struct Wide;
+template <> struct Wide<SV_DTYPE_BF16> {
+    static constexpr int SHIFT = 96;
+    static constexpr uint32_t SPECIAL = 0x7F80u;
+    static __device__ __forceinline__ double up() { return __hiloint2double((800 + 1023) << 20, 0); }
+    static __device__ __forceinline__ double lo(uint32_t w) { return __hiloint2double((int)(((w & 0x8000u) << 16) | ((w & 0x7FFFu) << 13)), 0); }
+    static __device__ __forceinline__ double hi(uint32_t w) { return __hiloint2double((int)((w & 0x80000000u) | ((w & 0x7FFF0000u) >> 3)), 0); }
+};
+template <> struct Wide<SV_DTYPE_FP16> {
+    static constexpr int SHIFT = 108;
+    static constexpr uint32_t SPECIAL = 0x7C00u;
+    static __device__ __forceinline__ double up() { return __hiloint2double((900 + 1023) << 20, 0); }
+    static __device__ __forceinline__ double lo(uint32_t w) { return __hiloint2double((int)(((w & 0x8000u) << 16) | ((w & 0x7FFFu) << 10)), 0); }
+    static __device__ __forceinline__ double hi(uint32_t w) { return __hiloint2double((int)((w & 0x80000000u) | ((w & 0x7FFF0000u) >> 6)), 0); }
 };
 
 /* Orders as the score does, NaN with minus infinity. */
@@ -37,182 +92,604 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
     const unsigned long long b = (unsigned long long)__double_as_longlong(s + 0.0);       /* -0 + 0 = +0: equal scores, equal keys */
     return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
+/* A float that orders as the key does (not strictly): the score's sign, its exponent brought back by SHIFT, 23 bits; what
+ * is too small is 0, what is too great (an infinity) the greatest float. */
+template <int SHIFT>
+__device__ __forceinline__ float key_float(uint32_t key_hi) {
+    const uint32_t b = (key_hi >> 31) ? key_hi & 0x7FFFFFFFu : ~key_hi & 0x7FFFFFFFu;
+    const int32_t e = (int32_t)b - ((896 - SHIFT) << 20);
+    const uint32_t f = e < 0 ? 0u : (uint32_t)min(e, (255 << 20) - 1) << 3;
+    return __uint_as_float(f | ((key_hi >> 31) ? 0u : 0x80000000u));
+}
 
-/* The `take` greatest of keys[0..m) (equal keys: the lower index), their indexes ascending into out; m > take > 0. */
-__device__ void select_keys(const unsigned long long* keys, uint32_t m, uint32_t take, uint32_t* out, uint32_t* hist /*[256 + 4]*/, uint32_t* warp_n /*[2][8]*/) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    unsigned long long known = 0, cut = 0;
-    uint32_t need = take;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += SP_THREADS) hist[i] = 0u;
-        __syncthreads();
-        for (uint32_t i = tid; i < m; i += SP_THREADS)
-            if ((keys[i] & known) == cut) atomicAdd(&hist[(uint32_t)(keys[i] >> shift) & 255u], 1u);
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t covered = 0u;
-            int b = 255;
-            for (; b > 0; --b) { if (covered + hist[b] >= need) break; covered += hist[b]; }
-            hist[256] = (uint32_t)b; hist[257] = need - covered;
-        }
-        __syncthreads();
-        cut |= (unsigned long long)hist[256] << shift; need = hist[257]; known |= 255ull << shift;
-        __syncthreads();
-    }
-    /* every key above the cut and the first `need` that equal it, in index order */
-    uint32_t done = 0u, ties = 0u;
-    for (uint32_t base = 0; base < m; base += SP_THREADS) {
-        const uint32_t i = base + tid;
-        const bool above = i < m && keys[i] > cut, equal = i < m && keys[i] == cut;
-        const unsigned eb = __ballot_sync(0xffffffffu, equal);
-        if (lane == 0) warp_n[warp] = __popc(eb);
-        __syncthreads();
-        uint32_t e = ties + __popc(eb & ((1u << lane) - 1u)), e_all = 0u;
-        for (int w = 0; w < SP_THREADS / 32; ++w) { if (w < warp) e += warp_n[w]; e_all += warp_n[w]; }
-        const bool in = above || (equal && e < need);
-        const unsigned ib = __ballot_sync(0xffffffffu, in);
-        if (lane == 0) warp_n[8 + warp] = __popc(ib);
-        __syncthreads();
-        uint32_t at = done + __popc(ib & ((1u << lane) - 1u)), n_all = 0u;
-        for (int w = 0; w < SP_THREADS / 32; ++w) { if (w < warp) at += warp_n[8 + w]; n_all += warp_n[8 + w]; }
-        if (in) out[at] = i;
-        done += n_all; ties += e_all;
-        __syncthreads();
+__device__ __forceinline__ void sp_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SP_THREADS) : "memory"); }
+
+struct SelectSmem {
+    uint32_t hist[SP_BINS];
+    unsigned long long list[SP_LIST];
+    unsigned long long cut;
+    uint32_t bin, need, in_bin, ties, n_list;
+    float lo[SP_WARPS], hi[SP_WARPS];
+    uint32_t warp_in[SP_WARPS], warp_tie[SP_WARPS];
+};
+
+/* A histogram walked down from its top bin by one warp: the bin where the count passes `need`, and what is still needed in it. */
+__device__ __forceinline__ void hist_walk(SelectSmem& S, uint32_t need, int lane) {
+    uint32_t mine = 0u;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) mine += S.hist[255 - 8 * lane - b];
+    uint32_t upto = mine;
+    for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
+    const unsigned reached = __ballot_sync(0xffffffffu, upto >= need);
+    if (lane == __ffs(reached) - 1) {
+        uint32_t covered = upto - mine, bin = 255u - 8u * (uint32_t)lane;
+        while (covered + S.hist[bin] < need) covered += S.hist[bin--];
+        S.bin = bin; S.need = need - covered; S.in_bin = S.hist[bin];
     }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(SP_THREADS) paged_sparse_kernel(const SparseParams P, const int D) {
-    using E = Elem<DT>;
-    extern __shared__ __align__(16) uint8_t sp_smem[];
-    const uint32_t kvh = blockIdx.x, r = blockIdx.y, keep = P.first + P.last + P.top;
-    double* qsum = (double*)sp_smem;                                             /* [D] */
-    unsigned long long* keys = (unsigned long long*)(qsum + D);                  /* [SP_CHUNK + top] */
-    uint32_t* key_id = (uint32_t*)(keys + SP_CHUNK + P.top);                      /* [SP_CHUNK + top] */
-    uint32_t* picked = key_id + SP_CHUNK + P.top;                                 /* [top] */
-    int32_t* ids = (int32_t*)(picked + P.top);                                    /* [keep] */
-    float* acc = (float*)(ids + keep);                                           /* [group][D] */
-    float* w = acc + P.group * D;                                                /* [group][16] */
-    float* ml = w + P.group * 16;                                                /* [group][3]: m, l, factor */
-    __shared__ uint32_t hist[260], warp_n[16];
-    __shared__ double part[SP_THREADS / 32];
+/* The `take` greatest of keys[0..m) (equal keys: the lower index), their indexes ascending into out; m > take > 0.  Called by
+ * SP_THREADS threads.
+ * First a histogram of 256 steps of equal width between the least and the greatest finite score: the bin that the last of the
+ * chosen falls in rarely holds more than a few (a tail of scores is thin), and those few are ranked against each other.  Where
+ * it holds more than SP_LIST — many equal scores — its keys are counted a byte at a time instead. */
+template <int SHIFT>
+__device__ __noinline__ void select_keys(const unsigned long long* keys, uint32_t m, uint32_t take, uint32_t* out, SelectSmem& S) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int32_t seq = P.row_seq[r];
-    if (seq < 0 || (uint32_t)seq >= P.seqs) { if (seq >= 0 && tid == 0 && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE); return; }
-    const int32_t p = P.row_pos[r];
-    const int32_t* row = P.table + (size_t)seq * P.stride;
-    const uint16_t* q = P.q + (size_t)r * P.q_stride + (size_t)kvh * P.group * D;
-    const size_t head0 = (size_t)r * P.q_heads + kvh * P.group;
-    int32_t* chosen = P.chosen ? P.chosen + ((size_t)r * P.kv_heads + kvh) * keep : nullptr;
-    if (p < 0) {
-        for (uint32_t i = tid; i < P.group * D; i += SP_THREADS) {
-            if (P.o) ((uint16_t*)P.o)[head0 * D + i] = 0;
-            if (P.res) { float* x = P.res + (head0 + i / D) * (D + 2); x[2 + i % D] = 0.f; if (i % D == 0) { x[0] = -INFINITY; x[1] = 0.f; } }
+    const uint32_t* key_hi = reinterpret_cast<const uint32_t*>(keys) + 1;
+    float mn = INFINITY, mx = -INFINITY;
+    for (uint32_t i = tid; i < m; i += SP_THREADS) {
+        const float f = key_float<SHIFT>(key_hi[2 * i]);
+        if (fabsf(f) < 3.0e38f) { mn = fminf(mn, f); mx = fmaxf(mx, f); }
+    }
+    for (int x = 16; x > 0; x >>= 1) { mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, x)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x)); }
+    if (lane == 0) { S.lo[warp] = mn; S.hi[warp] = mx; }
+    S.hist[tid] = 0u;
+    if (tid == 0) S.n_list = 0u;
+    sp_sync();
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; ++w) { mn = fminf(mn, S.lo[w]); mx = fmaxf(mx, S.hi[w]); }
+    if (!(mn < mx)) { mn = 0.f; mx = 0.f; }
+    const float per = mx > mn ? 255.99f / (mx - mn) : 0.f;
+    auto bin_of = [&](uint32_t i) { return (uint32_t)min(max((int)((key_float<SHIFT>(key_hi[2 * i]) - mn) * per), 0), 255); };
+    for (uint32_t i = tid; i < m; i += SP_THREADS) atomicAdd(&S.hist[bin_of(i)], 1u);
+    sp_sync();
+    if (warp == 0) hist_walk(S, take, lane);
+    sp_sync();
+    const uint32_t bin = S.bin, need = S.need, in_bin = S.in_bin;
+    /* keys of that bin above `cut`, and the first `ties` of those that equal it, belong to the choice */
+    if (in_bin == need) {
+        if (tid == 0) { S.cut = 0ull; S.ties = 0xFFFFFFFFu; }       /* the whole bin does (no key is 0 or less) */
+        sp_sync();
+    } else if (in_bin <= SP_LIST) {
+        for (uint32_t i = tid; i < m; i += SP_THREADS) if (bin_of(i) == bin) S.list[atomicAdd(&S.n_list, 1u)] = keys[i];
+        sp_sync();
+        if ((uint32_t)tid < in_bin) {
+            const unsigned long long k = S.list[tid];
+            uint32_t above = 0u, upto = 0u;
+            for (uint32_t j = 0; j < in_bin; ++j) { const unsigned long long x = S.list[j]; above += x > k; upto += x >= k; }
+            if (above < need && need <= upto) { S.cut = k; S.ties = need - above; }     /* equal keys write the same */
         }
-        if (chosen) for (uint32_t i = tid; i < keep; i += SP_THREADS) chosen[i] = -1;
+        sp_sync();
+    } else {
+        unsigned long long known = 0ull, cut = 0ull;
+        uint32_t left = need;
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            S.hist[tid] = 0u;
+            sp_sync();
+            for (uint32_t i = tid; i < m; i += SP_THREADS)
+                if ((keys[i] & known) == cut && bin_of(i) == bin) atomicAdd(&S.hist[(uint32_t)(keys[i] >> shift) & 255u], 1u);
+            sp_sync();
+            if (warp == 0) hist_walk(S, left, lane);
+            sp_sync();
+            cut |= (unsigned long long)S.bin << shift; left = S.need; known |= 255ull << shift;
+            sp_sync();
+        }
+        if (tid == 0) { S.cut = cut; S.ties = left; }
+        sp_sync();
+    }
+    /* in index order: each warp owns a run of indexes; one pass counts, one writes */
+    const unsigned long long cut = S.cut;
+    const uint32_t ties = S.ties, run = ((m + SP_THREADS - 1) / SP_THREADS) * 32u, i0 = warp * run, i1 = min(m, i0 + run);
+    uint32_t n_in = 0u, n_tie = 0u;
+    for (uint32_t i = i0 + lane; i < i0 + run; i += 32) {
+        bool in = false, tie = false;
+        if (i < i1) { const uint32_t b = bin_of(i); in = b > bin || (b == bin && keys[i] > cut); tie = b == bin && keys[i] == cut; }
+        n_in += __popc(__ballot_sync(0xffffffffu, in)); n_tie += __popc(__ballot_sync(0xffffffffu, tie));
+    }
+    if (lane == 0) { S.warp_in[warp] = n_in; S.warp_tie[warp] = n_tie; }
+    sp_sync();
+    uint32_t at = 0u, tied = 0u;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; ++w) if (w < warp) { at += S.warp_in[w]; tied += S.warp_tie[w]; }
+    at += min(tied, ties);
+    const unsigned below = (1u << lane) - 1u;
+    for (uint32_t i = i0 + lane; i < i0 + run; i += 32) {
+        bool in = false, tie = false;
+        if (i < i1) { const uint32_t b = bin_of(i); in = b > bin || (b == bin && keys[i] > cut); tie = b == bin && keys[i] == cut; }
+        const unsigned tb = __ballot_sync(0xffffffffu, tie);
+        in |= tie && tied + __popc(tb & below) < ties;
+        const unsigned ib = __ballot_sync(0xffffffffu, in);
+        if (in) out[at + __popc(ib & below)] = i;
+        at += __popc(ib); tied += __popc(tb);
+    }
+    sp_sync();
+}
+
+__device__ __forceinline__ void st_cluster_u64(const void* local, uint32_t rank, unsigned long long v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote), "l"(v) : "memory");
+}
+
+template <int D, int DT, int NHT>
+__global__ void __launch_bounds__(SP_THREADS + 32, D == 256 ? 1 : 2)
+paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const SparseParams P) {
+    using Cfg = SparseCfg<D>;
+    using E = Elem<DT>;
+    using W = Wide<DT>;
+    constexpr int HPB = 8 * NHT, KS = D / 16, NW = SP_WARPS, VS = KS / 2;      /* VS: 16-column steps of the value product a warp */
+    constexpr int Q_BYTES = Cfg::BOXES * HPB * 128;
+    constexpr bool QREG = NHT == 1;          /* 16 heads: the query's fragments are read from shared memory again for every tile */
+
+    extern __shared__ uint8_t sp_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)sp_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t keep = P.first + P.last + P.top;
+    uint8_t* ring = smem;
+    uint8_t* q_base = ring + Cfg::STAGES * Cfg::STAGE_BYTES;
+    uint64_t* full = (uint64_t*)(q_base + Q_BYTES);
+    uint64_t* empty = full + Cfg::STAGES;
+    volatile uint32_t* abort_flag = (volatile uint32_t*)(empty + Cfg::STAGES);
+    int32_t* slots = (int32_t*)(empty + Cfg::STAGES + 1);                         /* [keep] the chosen blocks' places in the pool */
+    uint32_t* ids = (uint32_t*)(slots + keep);                                    /* [top] the chosen blocks' numbers */
+    uint32_t* picked = ids + P.top;                                               /* [top] */
+    /* before the first tile the ring holds the scores */
+    unsigned long long* keys = (unsigned long long*)ring;                         /* [SP_CHUNK + top] */
+    double* qsum = (double*)(keys + SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX);     /* [D] */
+    SelectSmem& S = *(SelectSmem*)(qsum + D);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t CL = cluster_nctarank(), crank = cluster_ctarank();
+    const uint32_t unit = blockIdx.x / CL, hb = unit % P.head_blocks, kvh = (unit / P.head_blocks) % P.kv_heads, r = unit / P.head_blocks / P.kv_heads;
+    const uint32_t head0 = kvh * P.group + hb * HPB, heads = min((uint32_t)HPB, P.group - hb * HPB);
+
+    if (tid == 0) {
+        for (int s = 0; s < Cfg::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], NW); }
+        *abort_flag = 0u;
+        mbar_fence_init();
+        tma_prefetch_desc(&kmap); tma_prefetch_desc(&vmap);
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");      /* everything read below may be the work of the grid ahead */
+
+    const int32_t seq = P.row_seq[r], pos = P.row_pos[r];
+    if (seq < 0 || (uint32_t)seq >= P.seqs) { if (seq >= 0 && tid == 0 && crank == 0 && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE); return; }
+    const size_t out0 = (size_t)r * P.q_heads + head0;
+    int32_t* chosen = P.chosen && hb == 0 && crank == 0 ? P.chosen + ((size_t)r * P.kv_heads + kvh) * keep : nullptr;
+    if (pos < 0) {
+        if (crank != 0) return;
+        for (uint32_t i = tid; i < heads * D; i += blockDim.x) {
+            if (P.o) ((uint16_t*)P.o)[out0 * D + i] = 0;
+            if (P.res) { float* x = P.res + (out0 + i / D) * (D + 2); x[2 + i % D] = 0.f; if (i % D == 0) { x[0] = -INFINITY; x[1] = 0.f; } }
+        }
+        if (chosen) for (uint32_t i = tid; i < keep; i += blockDim.x) chosen[i] = -1;
         return;
     }
-    const PagedChoice c = paged_choice((uint32_t)p, P.block, P.first, P.last, P.top);
+    const PagedChoice c = paged_choice((uint32_t)pos, P.block, P.first, P.last, P.top);
+    const int32_t* row = P.table + (size_t)seq * P.stride;
+    const uint16_t* qrow = P.q + (size_t)r * P.q_stride;
     bool bad = false;
-    for (int e = tid; e < D; e += SP_THREADS) {
-        double s = 0;
-        for (uint32_t h = 0; h < P.group; ++h) s += (double)E::to_float(q[h * D + e]);
-        qsum[e] = s;
+
+    /* a peer's shared memory may be written only once the peer runs: arrive now, wait ahead of the first score */
+    if (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (warp < NW) {
+        for (int i = tid; i < HPB * (D / 8); i += SP_THREADS) {
+            const int h = i / (D / 8), j = i % (D / 8);
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if ((uint32_t)h < heads) x = *reinterpret_cast<const uint4*>(qrow + (size_t)(head0 + h) * D + j * 8);
+            *reinterpret_cast<uint4*>(q_base + (j / 8) * (HPB * 128) + swz128(h, j % 8)) = x;
+        }
+        if (c.take)
+            for (int e = tid; e < D; e += SP_THREADS) {
+                double s = 0;
+                for (uint32_t h = 0; h < P.group; ++h) s += (double)E::to_float(qrow[(size_t)(kvh * P.group + h) * D + e]);
+                qsum[e] = s * W::up();
+            }
     }
     __syncthreads();
-    uint32_t have = 0;                                                    /* the best so far, at the front of keys */
-    for (uint32_t base = c.lo; base < c.hi && c.take; base += SP_CHUNK) {
+    if (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+
+    /* ---- scores and choice, a chunk of blocks at a time ---- */
+    uint32_t have = 0;                                                    /* the best of the chunks so far: keys[0..have), ids[0..have) */
+    for (uint32_t base = c.lo; c.take && base < c.hi; base += SP_CHUNK) {
         const uint32_t n = min(SP_CHUNK, c.hi - base);
-        for (uint32_t i = warp; i < n; i += SP_THREADS / 32) {
-            const int32_t slot = paged_block_slot(row, P.stride, P.pool_pages, P.page_pos, P.block, base + i);
-            double s = 0;
-            if (slot >= 0) {
-                const uint16_t* m = P.means + ((size_t)((uint32_t)slot / P.block) * P.kv_heads + kvh) * D;
-                for (int e = lane; e < D; e += 32) s += qsum[e] * (double)E::to_float(m[e]);
-                for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            } else { s = -INFINITY; bad = true; }
-            if (lane == 0) { keys[have + i] = score_key(s); key_id[have + i] = base + i; }
+        if (warp < NW) {
+            double qd[Cfg::CPL][8];
+#pragma unroll
+            for (int x = 0; x < Cfg::CPL; ++x)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qd[x][e] = qsum[(x * Cfg::LPB + lane % Cfg::LPB) * 8 + e];
+            const uint32_t step = CL * NW * Cfg::WB;
+            const uint32_t i_lane = (crank * NW + warp) * Cfg::WB + lane;             /* the mean whose place lane `lane` looks up */
+            auto place = [&](uint32_t i) {
+                if (lane >= Cfg::WB || i >= n) return -1;
+                const int32_t s = paged_block_slot(row, P.stride, P.pool_pages, P.page_pos, P.block, base + i);
+                if (s < 0) { bad = true; return -1; }
+                return (int32_t)((uint32_t)s / P.block);
+            };
+            int32_t mine = place(i_lane);
+            for (uint32_t i0 = i_lane - lane; i0 < n; i0 += step) {
+                uint4 x[Cfg::U][Cfg::CPL];
+                bool there[Cfg::U];
+#pragma unroll
+                for (int u = 0; u < Cfg::U; ++u) {
+                    const int32_t m = __shfl_sync(0xffffffffu, mine, u * Cfg::BPS + lane / Cfg::LPB);
+                    there[u] = m >= 0;
+                    const uint4* src = reinterpret_cast<const uint4*>(P.means + ((size_t)(there[u] ? m : 0) * P.kv_heads + kvh) * D) + lane % Cfg::LPB;
+#pragma unroll
+                    for (int y = 0; y < Cfg::CPL; ++y) x[u][y] = there[u] ? __ldg(src + y * Cfg::LPB) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                mine = place(i0 + step + lane);
+                double s[Cfg::U];
+#pragma unroll
+                for (int u = 0; u < Cfg::U; ++u) {
+                    double a = 0;
+                    uint32_t special = 0u;
+#pragma unroll
+                    for (int y = 0; y < Cfg::CPL; ++y) {
+                        const uint32_t w[4] = {x[u][y].x, x[u][y].y, x[u][y].z, x[u][y].w};
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            a = fma(W::lo(w[z]), qd[y][2 * z], a); a = fma(W::hi(w[z]), qd[y][2 * z + 1], a);
+                            special = __vmaxu2(special, w[z] & 0x7FFF7FFFu);
+                        }
+                    }
+                    if ((special & 0xFFFFu) >= W::SPECIAL || (special >> 16) >= W::SPECIAL) {
+                        a = 0;
+#pragma unroll
+                        for (int y = 0; y < Cfg::CPL; ++y) {
+                            const uint32_t w[4] = {x[u][y].x, x[u][y].y, x[u][y].z, x[u][y].w};
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) { const float2 f = E::unpack2(w[z]); a += (double)f.x * qd[y][2 * z]; a += (double)f.y * qd[y][2 * z + 1]; }
+                        }
+                    }
+                    s[u] = a;
+                }
+                /* the lanes' parts of four means at once: each exchange halves what a lane still holds; whichever of two lanes adds,
+                 * the sum is the same */
+                constexpr int T0 = Cfg::LPB / 2, T1 = Cfg::LPB / 4;
+                const bool up0 = (lane & T0) != 0, up1 = (lane & T1) != 0;
+                double a0 = up0 ? s[2] : s[0], a1 = up0 ? s[3] : s[1];
+                a0 += __shfl_xor_sync(0xffffffffu, up0 ? s[0] : s[2], T0);
+                a1 += __shfl_xor_sync(0xffffffffu, up0 ? s[1] : s[3], T0);
+                double v = up1 ? a1 : a0;
+                v += __shfl_xor_sync(0xffffffffu, up1 ? a0 : a1, T1);
+#pragma unroll
+                for (int t = T1 / 2; t > 0; t >>= 1) v += __shfl_xor_sync(0xffffffffu, v, t);
+                const int u = (up0 ? 2 : 0) + (up1 ? 1 : 0);
+                const uint32_t i = i0 + u * Cfg::BPS + lane / Cfg::LPB;
+                bool is = false;
+#pragma unroll
+                for (int z = 0; z < Cfg::U; ++z) is = z == u ? there[z] : is;
+                if (i < n) {
+                    const unsigned long long k = score_key(is ? v : -INFINITY);
+                    if (CL == 1) { if (lane % T1 == 0) keys[have + i] = k; }
+                    else for (uint32_t to = lane % T1; to < CL; to += T1) st_cluster_u64(&keys[have + i], to, k);
+                }
+            }
         }
-        __syncthreads();
+        if (CL > 1) cluster_sync_all(); else __syncthreads();
         const uint32_t m = have + n;
-        if (m <= c.take) { have = m; continue; }
-        select_keys(keys, m, c.take, picked, hist, warp_n);
-        __syncthreads();
-        unsigned long long kk[4]; uint32_t ii[4];
-        for (uint32_t i = tid, u = 0; i < c.take; i += SP_THREADS, ++u) { kk[u] = keys[picked[i]]; ii[u] = key_id[picked[i]]; }
-        __syncthreads();
-        for (uint32_t i = tid, u = 0; i < c.take; i += SP_THREADS, ++u) { keys[i] = kk[u]; key_id[i] = ii[u]; }
-        __syncthreads();
-        have = c.take;
+        const bool more = base + SP_CHUNK < c.hi;
+        if (warp < NW) {
+            if (m <= c.take) {
+                for (uint32_t i = tid; i < n; i += SP_THREADS) ids[have + i] = base + i;
+            } else {
+                select_keys<W::SHIFT>(keys, m, c.take, picked, S);
+                /* the chosen move to the front, in order: read all, then write */
+                unsigned long long kk[SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS];
+                uint32_t ii[SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS];
+#pragma unroll
+                for (int z = 0; z < (int)(SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS); ++z) {
+                    const uint32_t i = tid + z * SP_THREADS;
+                    if (i < c.take) { const uint32_t at = picked[i]; kk[z] = keys[at]; ii[z] = at < have ? ids[at] : base + (at - have); }
+                }
+                sp_sync();
+#pragma unroll
+                for (int z = 0; z < (int)(SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS); ++z) {
+                    const uint32_t i = tid + z * SP_THREADS;
+                    if (i < c.take) { keys[i] = kk[z]; ids[i] = ii[z]; }
+                }
+            }
+        }
+        have = min(m, c.take);
+        if (more) { if (CL > 1) cluster_sync_all(); else __syncthreads(); }       /* no one writes the next scores over what a peer still reads */
     }
-    for (uint32_t i = tid; i < keep; i += SP_THREADS) {
+    __syncthreads();
+    for (uint32_t i = tid; i < keep; i += blockDim.x) {
         int32_t id = -1;
-        if (i < c.count) id = i < c.lo ? (int32_t)i : i < c.lo + c.take ? (int32_t)key_id[i - c.lo] : (int32_t)(c.hi + (i - c.lo - c.take));
-        ids[i] = id;
+        if (i < c.count) {
+            id = i < c.lo ? (int32_t)i : i < c.lo + c.take ? (int32_t)ids[i - c.lo] : (int32_t)(c.hi + (i - c.lo - c.take));
+            const int32_t slot = paged_block_slot(row, P.stride, P.pool_pages, P.page_pos, P.block, (uint32_t)id);
+            bad |= slot < 0;
+            /* a block whose page is none is asked for past the pool's last row, where TMA answers zeros */
+            slots[i] = slot < 0 ? (int32_t)(P.pool_pages * P.page_pos) : slot;
+        }
         if (chosen) chosen[i] = id;
     }
-    for (uint32_t i = tid; i < P.group * D; i += SP_THREADS) acc[i] = 0.f;
-    for (uint32_t h = tid; h < P.group; h += SP_THREADS) { ml[3 * h] = -INFINITY; ml[3 * h + 1] = 0.f; }
+    fence_proxy_async_smem();            /* the scores' accesses to the ring come before the loads into it */
     __syncthreads();
-    const uint32_t live = (c.count - 1u) * P.block + (uint32_t)p % P.block + 1u;       /* the row's own block is the last and may end early */
-    for (uint32_t t = 0; t < live; t += 16) {
-        const uint32_t n = min(16u, live - t);
-        const int32_t slot0 = paged_block_slot(row, P.stride, P.pool_pages, P.page_pos, P.block, (uint32_t)ids[t / P.block]);
-        bad |= slot0 < 0;
-        for (uint32_t i = tid; i < P.group * n; i += SP_THREADS) {
-            const uint32_t h = i / n, j = i % n;
-            float s = 0.f;
-            if (slot0 >= 0) {
-                const uint16_t* k = P.k + ((size_t)((uint32_t)slot0 + t % P.block + j) * P.kv_heads + kvh) * D;
-                for (int e = 0; e < D; ++e) s += E::to_float(q[h * D + e]) * E::to_float(k[e]);
+
+    /* ---- attend: tile t of the chosen positions belongs to thread block t % CL ---- */
+    const uint32_t live = (c.count - 1u) * P.block + (uint32_t)pos % P.block + 1u;      /* the row's own block is the last and may end early */
+    const uint32_t tiles = (live + 63u) / 64u;
+    const int nt = tiles > crank ? (int)((tiles - crank + CL - 1) / CL) : 0;
+
+    float m_run[NHT][2], l_run[NHT][2], oacc[NHT][VS][4];
+#pragma unroll
+    for (int n = 0; n < NHT; ++n) {
+        m_run[n][0] = m_run[n][1] = -INFINITY; l_run[n][0] = l_run[n][1] = 0.f;
+#pragma unroll
+        for (int k = 0; k < VS; ++k) { oacc[n][k][0] = oacc[n][k][1] = oacc[n][k][2] = oacc[n][k][3] = 0.f; }
+    }
+    if (warp == NW) {
+        /* ---- the loads: one box of 64 columns by min(B, 64) positions a lane ---- */
+        const uint32_t br = min(P.block, 64u), sub = 64u / br;
+        const uint64_t pol = l2_policy_evict_first();
+        for (int it = 0; it < nt; ++it) {
+            const int s = it % Cfg::STAGES;
+            if (it >= Cfg::STAGES && !mbar_wait(&empty[s], ((it / Cfg::STAGES) - 1) & 1, abort_flag, P.status)) break;
+            const uint32_t p0 = (crank + it * CL) * 64u;
+            const uint32_t boxes = min(sub, (live - p0 + br - 1u) / br);
+            uint8_t* st = ring + s * Cfg::STAGE_BYTES;
+            if (lane == 0) mbar_expect_tx(&full[s], boxes * br * 128u * Cfg::BOXES * 2u);
+            __syncwarp();
+            for (uint32_t i = lane; i < boxes * Cfg::BOXES * 2u; i += 32) {
+                const uint32_t b = i / (Cfg::BOXES * 2u), x = i % (Cfg::BOXES * 2u), col = x % Cfg::BOXES;
+                const uint32_t at = p0 + b * br;
+                const int32_t y = slots[at / P.block] + (int32_t)(at % P.block);
+                tma_load_2d_hint(st + (x / Cfg::BOXES) * Cfg::K_BYTES + col * Cfg::BOX_BYTES + b * br * 128u, x < Cfg::BOXES ? (const void*)&kmap : (const void*)&vmap, &full[s],
+                                 (int32_t)(kvh * D + col * 64u), y, pol);
             }
-            w[h * 16 + j] = s * P.scale;
+            __syncwarp();
         }
-        __syncthreads();
-        for (uint32_t h = tid; h < P.group; h += SP_THREADS) {
-            float m = ml[3 * h];
-            for (uint32_t j = 0; j < n; ++j) m = fmaxf(m, w[h * 16 + j]);
-            const float u = m == -INFINITY ? 0.f : m, f = expf(ml[3 * h] - u);
-            float l = ml[3 * h + 1] * f;
-            for (uint32_t j = 0; j < n; ++j) { w[h * 16 + j] = expf(w[h * 16 + j] - u); l += w[h * 16 + j]; }
-            ml[3 * h] = m; ml[3 * h + 1] = l; ml[3 * h + 2] = f;
+    } else {
+        const uint32_t q_u32 = smem_u32(q_base);
+        auto load_qfrag = [&](int n, int kk, uint32_t& b0, uint32_t& b1) {
+            /* B fragment of Q^T for heads n*8..n*8+7, columns kk*16..+15: two 8x8 blocks (chunks 2kk, 2kk+1) */
+            const int chunk = 2 * kk + ((lane >> 3) & 1), hrow = n * 8 + (lane & 7);
+            uint32_t r2, r3;
+            ldsm_x4(q_u32 + (chunk / 8) * (HPB * 128) + swz128(hrow, chunk % 8), b0, b1, r2, r3);
+        };
+        uint32_t qf[QREG ? KS : 1][2];
+        if (QREG) {
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) load_qfrag(0, kk, qf[kk][0], qf[kk][1]);
         }
-        __syncthreads();
-        for (uint32_t i = tid; i < P.group * D; i += SP_THREADS) {
-            const uint32_t h = i / D, e = i % D;
-            float a = acc[i] * ml[3 * h + 2];
-            if (slot0 >= 0)
-                for (uint32_t j = 0; j < n; ++j) a += w[h * 16 + j] * E::to_float(P.v[((size_t)((uint32_t)slot0 + t % P.block + j) * P.kv_heads + kvh) * D + e]);
-            acc[i] = a;
+        const int r_lo = lane >> 2, w4 = warp & 3, half = warp >> 2;      /* positions [16 w4, +16) of a tile, value columns [half D/2, +D/2) */
+        for (int it = 0; it < nt; ++it) {
+            const int s = it % Cfg::STAGES;
+            if (!mbar_wait(&full[s], (it / Cfg::STAGES) & 1, abort_flag, P.status)) break;
+            uint8_t* stage = ring + s * Cfg::STAGE_BYTES;
+            const uint32_t kst = smem_u32(stage), vst = kst + Cfg::K_BYTES;
+            const uint32_t p0 = (crank + it * CL) * 64u + w4 * 16u;
+            /* rows of V behind the row's own position may hold anything: zero, so that a zero weight times a NaN cannot reach the sum */
+            if (p0 + 16u > live) {
+                for (int i = lane; i < 16 * (D / 16); i += 32) {
+                    const int y = i / (D / 16), j = half * (D / 16) + i % (D / 16);
+                    if (p0 + y >= live)
+                        *reinterpret_cast<uint4*>(stage + Cfg::K_BYTES + (j / 8) * Cfg::BOX_BYTES + swz128(w4 * 16 + y, j % 8)) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                __syncwarp();
+            }
+            /* S^T[16 positions][heads] = K_tile Q^T, two interleaved accumulators per head tile */
+            float sa[NHT][4], sb[NHT][4];
+#pragma unroll
+            for (int n = 0; n < NHT; ++n) { sa[n][0] = sa[n][1] = sa[n][2] = sa[n][3] = 0.f; sb[n][0] = sb[n][1] = sb[n][2] = sb[n][3] = 0.f; }
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                const int krow = w4 * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, chunk = 2 * kk + (lane >> 4);
+                uint32_t a0, a1, a2, a3;
+                ldsm_x4(kst + (chunk / 8) * Cfg::BOX_BYTES + swz128(krow, chunk % 8), a0, a1, a2, a3);
+#pragma unroll
+                for (int n = 0; n < NHT; ++n) {
+                    uint32_t b0, b1;
+                    if (QREG) { b0 = qf[kk][0]; b1 = qf[kk][1]; } else load_qfrag(n, kk, b0, b1);
+                    if (kk & 1) mma16816<DT>(sb[n], a0, a1, a2, a3, b0, b1);
+                    else        mma16816<DT>(sa[n], a0, a1, a2, a3, b0, b1);
+                }
+            }
+            /* online softmax over positions (accumulator rows), per head (accumulator columns).  The weights go to the MMA as
+             * two 16-bit parts, value and what its rounding left: the tensor pipe is a sixth busy, and one part alone would
+             * double the answer's rounding error */
+            uint32_t ph[NHT][2], pl[NHT][2];
+            const bool v0 = p0 + r_lo < live, v1 = p0 + r_lo + 8 < live;
+#pragma unroll
+            for (int n = 0; n < NHT; ++n) {
+                const float t0 = v0 ? (sa[n][0] + sb[n][0]) * P.scale_log2 : -INFINITY;   /* position r_lo,   head A */
+                const float t1 = v0 ? (sa[n][1] + sb[n][1]) * P.scale_log2 : -INFINITY;   /* position r_lo,   head B */
+                const float t2 = v1 ? (sa[n][2] + sb[n][2]) * P.scale_log2 : -INFINITY;   /* position r_lo+8, head A */
+                const float t3 = v1 ? (sa[n][3] + sb[n][3]) * P.scale_log2 : -INFINITY;   /* position r_lo+8, head B */
+                float ma = fmaxf(t0, t2), mb = fmaxf(t1, t3);
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                    ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, x));
+                    mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, x));
+                }
+                const float na = fmaxf(m_run[n][0], ma), nb = fmaxf(m_run[n][1], mb);
+                const float ua = (na == -INFINITY) ? 0.f : na, ub = (nb == -INFINITY) ? 0.f : nb;
+                const float fa = fast_exp2(m_run[n][0] - ua), fb = fast_exp2(m_run[n][1] - ub);
+                m_run[n][0] = na; m_run[n][1] = nb;
+                const float e0 = fast_exp2(t0 - ua), e1 = fast_exp2(t1 - ub), e2 = fast_exp2(t2 - ua), e3 = fast_exp2(t3 - ub);
+                const uint32_t w0 = E::pack2(e0, e1), w1 = E::pack2(e2, e3);
+                const float2 f0 = E::unpack2(w0), f1 = E::unpack2(w1);
+                ph[n][0] = movm_t(w0); ph[n][1] = movm_t(w1);
+                pl[n][0] = movm_t(E::pack2(e0 - f0.x, e1 - f0.y)); pl[n][1] = movm_t(E::pack2(e2 - f1.x, e3 - f1.y));
+                l_run[n][0] = l_run[n][0] * fa + (e0 + e2);
+                l_run[n][1] = l_run[n][1] * fb + (e1 + e3);
+                if (__any_sync(0xffffffffu, fa != 1.f || fb != 1.f)) {
+#pragma unroll
+                    for (int k = 0; k < VS; ++k) { oacc[n][k][0] *= fa; oacc[n][k][2] *= fa; oacc[n][k][1] *= fb; oacc[n][k][3] *= fb; }
+                }
+            }
+            /* O^T[value column][head] += V_tile^T P^T */
+#pragma unroll
+            for (int mt = 0; mt < VS; ++mt) {
+                const int j = lane >> 3, vrow = w4 * 16 + (lane & 7) + (j >> 1) * 8, chunk = 2 * (half * VS + mt) + (j & 1);
+                uint32_t a0, a1, a2, a3;
+                ldsm_x4_t(vst + (chunk / 8) * Cfg::BOX_BYTES + swz128(vrow, chunk % 8), a0, a1, a2, a3);
+#pragma unroll
+                for (int n = 0; n < NHT; ++n) {
+                    mma16816<DT>(oacc[n][mt], a0, a1, a2, a3, ph[n][0], ph[n][1]);
+                    mma16816<DT>(oacc[n][mt], a0, a1, a2, a3, pl[n][0], pl[n][1]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
         }
+        /* the lanes that share a head column hold disjoint positions: fold their sums */
+#pragma unroll
+        for (int n = 0; n < NHT; ++n)
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                l_run[n][0] += __shfl_xor_sync(0xffffffffu, l_run[n][0], x);
+                l_run[n][1] += __shfl_xor_sync(0xffffffffu, l_run[n][1], x);
+            }
+    }
+
+    /* ---- the warps' partials meet in shared memory (the ring is free now), then the cluster's thread blocks ---- */
+    __syncthreads();
+    if (*abort_flag != 0u) {
+        /* a wait gave up (the status word says so): copies asked for may still be on their way into the ring, so every stage gets
+         * a bounded chance to land before the ring is written over */
+        if (tid == 0)
+            for (int s = 0; s < Cfg::STAGES && s < nt; ++s) {
+                const int last = (nt - 1 - s) / Cfg::STAGES;
+                for (uint32_t i = 0; i < (1u << 16) && !mbar_try_wait(&full[s], last & 1); ++i) {}
+            }
         __syncthreads();
     }
+    constexpr int PW = NW / 2;                        /* warps that split a tile by positions */
+    float* wm = (float*)ring;                         /* [PW][HPB] */
+    float* wl = wm + PW * HPB;                        /* [PW][HPB] */
+    float* wo = wl + PW * HPB;                        /* [PW][HPB][D] */
+    float* bacc = wo + (size_t)PW * HPB * D;          /* [HPB][D] */
+    float* bm = bacc + HPB * D;                       /* [HPB] log2 units */
+    float* bl = bm + HPB;                             /* [HPB] */
+    if (warp < NW) {
+        const int r_lo = lane >> 2, c2 = (lane & 3) * 2, w4 = warp & 3, half = warp >> 2;
+#pragma unroll
+        for (int n = 0; n < NHT; ++n) {
+            const int ha = n * 8 + c2;
+            if (r_lo == 0 && half == 0) {
+                wm[w4 * HPB + ha] = m_run[n][0]; wm[w4 * HPB + ha + 1] = m_run[n][1];
+                wl[w4 * HPB + ha] = l_run[n][0]; wl[w4 * HPB + ha + 1] = l_run[n][1];
+            }
+#pragma unroll
+            for (int k = 0; k < VS; ++k) {
+                float* at = wo + (size_t)(w4 * HPB) * D + (half * VS + k) * 16 + r_lo;
+                at[(ha) * D] = oacc[n][k][0];
+                at[(ha + 1) * D] = oacc[n][k][1];
+                at[(ha) * D + 8] = oacc[n][k][2];
+                at[(ha + 1) * D + 8] = oacc[n][k][3];
+            }
+        }
+    }
+    __syncthreads();
     bool hit = false;
-    for (uint32_t i = tid; i < P.group * D; i += SP_THREADS) {
+    auto answer = [&](uint32_t h, uint32_t e, float m, float l, float acc) {
+        const size_t hq = out0 + h;
+        if (P.o) ((uint16_t*)P.o)[hq * D + e] = E::from_float(acc / l, hit);
+        if (P.res) { float* x = P.res + hq * (D + 2); x[2 + e] = acc; if (e == 0) { x[0] = m * SV_LN2; x[1] = l; } }
+    };
+    for (uint32_t i = tid; i < heads * D; i += blockDim.x) {
         const uint32_t h = i / D, e = i % D;
-        if (P.o) ((uint16_t*)P.o)[head0 * D + i] = E::from_float(acc[i] / ml[3 * h + 1], hit);
-        if (P.res) { float* x = P.res + (head0 + h) * (D + 2); x[2 + e] = acc[i]; if (e == 0) { x[0] = ml[3 * h]; x[1] = ml[3 * h + 1]; } }
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PW; ++w) m = fmaxf(m, wm[w * HPB + h]);
+        float acc = 0.f, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < PW; ++w) {
+            const float mw = wm[w * HPB + h];
+            if (mw != -INFINITY) { const float f = fast_exp2(mw - m); acc += wo[(size_t)(w * HPB + h) * D + e] * f; l += wl[w * HPB + h] * f; }
+        }
+        if (CL == 1) answer(h, e, m, l, acc);
+        else { bacc[i] = acc; if (e == 0) { bm[h] = m; bl[h] = l; } }
+    }
+    if (CL > 1) {
+        cluster_sync_all();
+        /* thread block c folds columns [c D/CL, (c+1) D/CL) of every head over all, in order */
+        const uint32_t DS = D / CL;
+        for (uint32_t i = tid; i < heads * DS; i += blockDim.x) {
+            const uint32_t h = i / DS, e = crank * DS + i % DS;
+            float pm[16], pl[16], pa[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                if (x < (int)CL) { pm[x] = ld_cluster_f32(bm + h, x); pl[x] = ld_cluster_f32(bl + h, x); pa[x] = ld_cluster_f32(bacc + h * D + e, x); }
+            float m = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) if (x < (int)CL) m = fmaxf(m, pm[x]);
+            float acc = 0.f, l = 0.f;
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                if (x < (int)CL && pm[x] != -INFINITY) { const float f = fast_exp2(pm[x] - m); acc += pa[x] * f; l += pl[x] * f; }
+            answer(h, e, m, l, acc);
+        }
+        cluster_sync_all();                           /* a peer's shared memory is there until all have read it */
     }
     if (hit && P.over) atomicOr(P.over, SV_FAULT_OVERFLOW);
     if (bad && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE);
-    (void)part;
 }
 
-static cudaError_t sparse_launch(const SparseParams& P, uint32_t rows, uint32_t d, int dtype, cudaStream_t st) {
-    const size_t smem = 8 * d + 12 * (SP_CHUNK + (size_t)P.top) + 4 * (size_t)P.top + 4 * (size_t)(P.first + P.last + P.top) + 4 * (size_t)P.group * (d + 19);
+template <int D, int DT, int NHT>
+static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& vm, const SparseParams& P, uint64_t units, uint32_t cluster, cudaStream_t st) {
+    using Cfg = SparseCfg<D>;
+    const uint32_t keep = P.first + P.last + P.top;
+    const size_t fixed = 1024 + (size_t)Cfg::STAGES * Cfg::STAGE_BYTES + Cfg::BOXES * 8 * NHT * 128 + (2 * Cfg::STAGES + 1) * 8;
+    const size_t smem = fixed + ((size_t)keep + 2 * P.top) * 4;
+    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX) * 8 + D * 8 + sizeof(SelectSmem), "the scores fit the ring");
+    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (size_t)(SP_WARPS / 2 + 1) * 8 * NHT * (D + 2) * 4, "the partials fit the ring");
     static std::atomic<bool> attr_set[SPARSE_DEVICES];
-    int dev = 0; cudaGetDevice(&dev);
-    if (dev >= 0 && dev < SPARSE_DEVICES && !attr_set[dev].load(std::memory_order_acquire)) {
-        cudaError_t e = cudaFuncSetAttribute(paged_sparse_kernel<SV_DTYPE_FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_sparse_kernel<SV_DTYPE_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    int d = 0; cudaGetDevice(&d);
+    if (d >= 0 && d < SPARSE_DEVICES && !attr_set[d].load(std::memory_order_acquire)) {
+        cudaError_t e = cudaFuncSetAttribute(paged_sparse_kernel<D, DT, NHT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + 3 * SILVANN_B200_PAGED_KEEP_MAX * 4));
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_sparse_kernel<D, DT, NHT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
-        attr_set[dev].store(true, std::memory_order_release);
+        attr_set[d].store(true, std::memory_order_release);
     }
-    const dim3 grid(P.kv_heads, rows);
-    if (dtype == SV_DTYPE_FP16) paged_sparse_kernel<SV_DTYPE_FP16><<<grid, SP_THREADS, smem, st>>>(P, (int)d);
-    else paged_sparse_kernel<SV_DTYPE_BF16><<<grid, SP_THREADS, smem, st>>>(P, (int)d);
-    note_launch(1);
-    return cudaGetLastError();
+    cudaError_t e = cudaErrorInvalidValue;
+    for (; cluster > 0; cluster /= 2) {               /* a cluster that the card cannot place goes out again half as large */
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(units * cluster)); cfg.blockDim = dim3(SP_THREADS + 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+        cudaLaunchAttribute at[2];
+        unsigned na = 0;
+        if (cluster > 1u) { at[na].id = cudaLaunchAttributeClusterDimension; at[na].val.clusterDim.x = cluster; at[na].val.clusterDim.y = 1; at[na].val.clusterDim.z = 1; ++na; }
+        if (pdl_allowed()) { at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[na].val.programmaticStreamSerializationAllowed = 1; ++na; }
+        cfg.attrs = at; cfg.numAttrs = na;
+        e = cudaLaunchKernelEx(&cfg, paged_sparse_kernel<D, DT, NHT>, km, vm, P);
+        if (e == cudaSuccess) { note_launch(1); return cudaGetLastError(); }
+        (void)cudaGetLastError();
+    }
+    return e;
+}
+
+static cudaError_t sparse_launch(SparseParams& P, const void* k, const void* v, uint32_t rows, uint32_t d, int dtype, cudaStream_t st) {
+    const uint32_t nht = P.group <= 8u ? 1u : 2u;
+    P.head_blocks = (P.group + 8u * nht - 1u) / (8u * nht);
+    const uint64_t units = (uint64_t)rows * P.kv_heads * P.head_blocks, cols = (uint64_t)P.kv_heads * d;
+    /* As many thread blocks a row as keep every SM busy once (twice where two fit one), as far as a row's longest list of tiles goes round. */
+    const uint32_t sms = device_sm_count() * (d == 256 ? 1u : 2u), tiles = ((P.first + P.last + P.top) * P.block + 63u) / 64u;
+    uint32_t cluster = 1u;
+    while (cluster < 16u && units * cluster * 2u <= sms && cluster < tiles) cluster *= 2u;
+    CUtensorMap km, vm;
+    const bool bf = dtype == SV_DTYPE_BF16;
+    const uint32_t box = P.block < 64u ? P.block : 64u;
+    if (!make_map_2d_sw128(&km, k, cols, (uint64_t)P.pool_pages * P.page_pos, cols * 2u, 64u, box, bf) || !make_map_2d_sw128(&vm, v, cols, (uint64_t)P.pool_pages * P.page_pos, cols * 2u, 64u, box, bf))
+        return cudaErrorInvalidValue;
+#define SV_SPARSE_CASE(DD, TT) return nht == 1u ? sparse_launch_one<DD, TT, 1>(km, vm, P, units, cluster, st) : sparse_launch_one<DD, TT, 2>(km, vm, P, units, cluster, st)
+    if (!bf) { if (d == 64) SV_SPARSE_CASE(64, SV_DTYPE_FP16); else if (d == 128) SV_SPARSE_CASE(128, SV_DTYPE_FP16); else SV_SPARSE_CASE(256, SV_DTYPE_FP16); }
+    else { if (d == 64) SV_SPARSE_CASE(64, SV_DTYPE_BF16); else if (d == 128) SV_SPARSE_CASE(128, SV_DTYPE_BF16); else SV_SPARSE_CASE(256, SV_DTYPE_BF16); }
+#undef SV_SPARSE_CASE
 }
 
 }  // namespace sv
@@ -228,9 +705,9 @@ SV_EXPORT int silvann_b200_paged_sparse(void* o, float* res, int32_t* chosen, co
     if ((!o && !res) || !q || !k_pool || !v_pool || (top && !k_means) || !row_seq || !row_pos || !page_table) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_sparse: a null operand");
     if (dtype != SILVANN_B200_DTYPE_FP16 && dtype != SILVANN_B200_DTYPE_BF16) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_sparse: dtype %d", dtype);
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_sparse: head_dim %u (64, 128 or 256)", head_dim);
-    if (kv_heads == 0 || kv_heads > 65535u || q_heads == 0 || q_heads % kv_heads != 0 || q_heads / kv_heads > 64u)
+    if (kv_heads == 0 || kv_heads > 4096u || q_heads == 0 || q_heads % kv_heads != 0 || q_heads / kv_heads > 64u)
         return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_sparse: %u query heads over %u kv heads (up to 64 each)", q_heads, kv_heads);
-    if (rows == 0 || rows > 65535u || seqs == 0 || table_stride == 0) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_sparse: %u rows, %u sequences of %u table columns", rows, seqs, table_stride);
+    if (rows == 0 || rows > (1u << 24) / kv_heads || seqs == 0 || table_stride == 0) return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_sparse: %u rows, %u sequences of %u table columns", rows, seqs, table_stride);
     if (pool_pages == 0 || page_positions == 0 || pool_pages > 0x7FFFFFFFull / page_positions)
         return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_sparse: pool of %llu pages of %u positions", (unsigned long long)pool_pages, page_positions);
     if ((block_positions != 16 && block_positions != 32 && block_positions != 64 && block_positions != 128) || page_positions % block_positions)
@@ -244,11 +721,11 @@ SV_EXPORT int silvann_b200_paged_sparse(void* o, float* res, int32_t* chosen, co
         return sv_ext_fail(SILVANN_B200_E_ARGUMENT, "paged_sparse: an operand's alignment is outside the kernel's fit");
     sv::SparseParams P;
     memset(&P, 0, sizeof P);
-    P.o = o; P.res = res; P.chosen = chosen; P.q = (const uint16_t*)q; P.k = (const uint16_t*)k_pool; P.v = (const uint16_t*)v_pool; P.means = (const uint16_t*)k_means;
+    P.o = o; P.res = res; P.chosen = chosen; P.q = (const uint16_t*)q; P.means = (const uint16_t*)k_means;
     P.row_seq = row_seq; P.row_pos = row_pos; P.table = page_table; P.over = over; P.status = sv::device_status_word(); P.q_stride = q_stride; P.seqs = seqs;
     P.stride = table_stride; P.pool_pages = (uint32_t)pool_pages; P.page_pos = page_positions; P.block = block_positions; P.q_heads = q_heads; P.kv_heads = kv_heads;
-    P.group = q_heads / kv_heads; P.first = first; P.last = last; P.top = top; P.scale = 1.0f / sqrtf((float)head_dim);
-    cudaError_t e = sv::sparse_launch(P, rows, head_dim, dtype, (cudaStream_t)stream);
+    P.group = q_heads / kv_heads; P.first = first; P.last = last; P.top = top; P.scale_log2 = (1.0f / sqrtf((float)head_dim)) * SV_LOG2E;
+    cudaError_t e = sv::sparse_launch(P, k_pool, v_pool, rows, head_dim, dtype, (cudaStream_t)stream);
     if (e == cudaSuccess) return SILVANN_B200_OK;
     (void)cudaGetLastError();
     return sv_ext_fail(SILVANN_B200_E_CUDA, "paged_sparse: launch: %s", cudaGetErrorString(e));

@@ -408,6 +408,21 @@ def test_sparse_bad_pages(cuda):
     P.check([1], [120], 8, 1, 2, 4, got, short)
 
 
+@pytest.mark.parametrize("d,kvh,block,rows,keep", [(128, 1, 128, 20, (1, 1, 14)), (128, 2, 32, 10, (2, 2, 60)), (64, 4, 16, 5, (1, 2, 61)), (256, 1, 64, 10, (1, 2, 29))])
+def test_sparse_many_rows_with_many_tiles_each(cuda, d, kvh, block, rows, keep):
+    """Rows enough that each is one thread block's, which goes round its ring of tiles many times."""
+    lens = [2900 - 37 * s for s in range(8)]
+    P = Paged(cuda, 28, lens, kvh, d, 1, block, block)
+    seq = [s for s in range(8) for _ in range(rows)]
+    pos = [lens[s] - 1 - 11 * j for s in range(8) for j in range(rows)]
+    got = P.run(seq, pos, 8 * kvh, *keep)
+    again = P.run(seq, pos, 8 * kvh, *keep, q=got[0].reshape(len(seq), -1))
+    assert ext.device_status() == 0
+    for x, y in zip(got[1:], again[1:]):
+        assert np.array_equal(x, y)
+    P.check(seq, pos, 8 * kvh, *keep, got)
+
+
 def test_sparse_without_scores_needs_no_means(cuda):
     P = Paged(cuda, 25, [500, 20], 2, 64, 1, 64, 64)
     got = P.run([0, 1], [499, 19], 4, 2, 2, 0, means=False)
