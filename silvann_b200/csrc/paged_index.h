@@ -18,11 +18,22 @@ SV_HD int32_t paged_page(const int32_t* row, uint32_t stride, uint32_t pool_page
     return (page < 0 || (uint32_t)page >= pool_pages) ? -1 : page;
 }
 
-/* The first pool position of block `block` of a sequence (`block_pos` positions, a divisor of a page's), or -1. */
-SV_HD int32_t paged_block_slot(const int32_t* row, uint32_t stride, uint32_t pool_pages, uint32_t page_pos, uint32_t block_pos, uint32_t block) {
-    const uint32_t per = page_pos / block_pos, col = block / per;
+/* Division by a number that stays the same through a launch: a multiply and a shift, for numerators below 2^31. */
+struct PagedDiv { uint32_t d, mul, shift; };
+SV_HD PagedDiv paged_div(uint32_t d) {
+    PagedDiv x;
+    x.d = d; x.shift = 0;
+    while (x.shift < 31u && (1u << x.shift) < d) ++x.shift;
+    x.mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << x.shift) - d)) / d + 1u);
+    return x;
+}
+SV_HD uint32_t paged_quot(uint32_t n, const PagedDiv& x) { return ((uint32_t)(((uint64_t)n * x.mul) >> 32) + n) >> x.shift; }
+
+/* The number in the pool of block `block` of a sequence (a page holds per.d of them), or -1. */
+SV_HD int32_t paged_block(const int32_t* row, uint32_t stride, uint32_t pool_pages, const PagedDiv& per, uint32_t block) {
+    const uint32_t col = paged_quot(block, per);
     const int32_t page = paged_page(row, stride, pool_pages, col);
-    return page < 0 ? -1 : (int32_t)((uint32_t)page * page_pos + (block - col * per) * block_pos);
+    return page < 0 ? -1 : (int32_t)((uint32_t)page * per.d + (block - col * per.d));
 }
 
 /* How a row at position p splits its n = p / B + 1 blocks: the first `lo` and those from `hi` on are always attended, and of

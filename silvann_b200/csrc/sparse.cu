@@ -34,11 +34,11 @@ namespace svf { extern std::atomic<uint64_t> g_counters[SILVANN_B200_COUNTERS]; 
 namespace sv {
 
 static constexpr int SPARSE_DEVICES = 64;
-#define SP_WARPS 8                            /* warps that score, choose and multiply; one more issues the loads */
+#define SP_WARPS 8
 #define SP_THREADS (SP_WARPS * 32)
 #define SP_CHUNK 4096u                        /* scores looked at in one go; the best of the chunks before them ride along */
-#define SP_BINS 256u
-#define SP_LIST 128u
+#define SP_CAP (SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX)
+#define SP_LIST 256u                          /* one thread each */
 
 template <int D> struct SparseCfg {
     static constexpr int BOXES = D / 64;                  /* 64-column (128-byte) boxes a row */
@@ -50,7 +50,7 @@ template <int D> struct SparseCfg {
     static constexpr int LPB = D == 256 ? 16 : 8;
     static constexpr int CPL = D / 8 / LPB;
     static constexpr int BPS = 32 / LPB;
-    static constexpr int U = 4;
+    static constexpr int U = 8;
     static constexpr int WB = BPS * U;
 };
 
@@ -62,6 +62,7 @@ struct SparseParams {
     const int32_t *row_seq, *row_pos, *table;
     unsigned int *over, *status;
     uint64_t q_stride;
+    PagedDiv per;                       /* blocks a page */
     uint32_t seqs, stride, pool_pages, page_pos, block, q_heads, kv_heads, group, head_blocks, first, last, top;
     float scale_log2;
 };
@@ -95,110 +96,142 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 /* A float that orders as the key does (not strictly): the score's sign, its exponent brought back by SHIFT, 23 bits; what
  * is too small is 0, what is too great (an infinity) the greatest float. */
 template <int SHIFT>
-__device__ __forceinline__ float key_float(uint32_t key_hi) {
-    const uint32_t b = (key_hi >> 31) ? key_hi & 0x7FFFFFFFu : ~key_hi & 0x7FFFFFFFu;
+__device__ __forceinline__ float key_float(unsigned long long key) {
+    const uint32_t k = (uint32_t)(key >> 32), b = (k >> 31) ? k & 0x7FFFFFFFu : ~k & 0x7FFFFFFFu;
     const int32_t e = (int32_t)b - ((896 - SHIFT) << 20);
     const uint32_t f = e < 0 ? 0u : (uint32_t)min(e, (255 << 20) - 1) << 3;
-    return __uint_as_float(f | ((key_hi >> 31) ? 0u : 0x80000000u));
+    return __uint_as_float(f | ((k >> 31) ? 0u : 0x80000000u));
 }
 
-__device__ __forceinline__ void sp_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SP_THREADS) : "memory"); }
-
-struct SelectSmem {
-    uint32_t hist[SP_BINS];
-    unsigned long long list[SP_LIST];
+/* What the ring holds before the first tile: the scores of a chunk of blocks behind the best of the chunks before, and the
+ * choice's own tables. */
+struct ChoiceSmem {
+    unsigned long long keys[SP_CAP];
+    unsigned long long list_key[SP_LIST];
+    int32_t place[SP_CAP];                 /* the block's number in the pool, -1: none */
+    uint32_t hist[256];
+    uint32_t list[SP_LIST], sure[SP_LIST];
+    uint32_t ids[SILVANN_B200_PAGED_KEEP_MAX], picked[SILVANN_B200_PAGED_KEEP_MAX];
+    double qsum[256];
     unsigned long long cut;
-    uint32_t bin, need, in_bin, ties, n_list;
     float lo[SP_WARPS], hi[SP_WARPS];
     uint32_t warp_in[SP_WARPS], warp_tie[SP_WARPS];
+    uint32_t bin, need, in_bin, ties, n_list, n_sure;
+    uint8_t bins[SP_CAP];
 };
 
-/* A histogram walked down from its top bin by one warp: the bin where the count passes `need`, and what is still needed in it. */
-__device__ __forceinline__ void hist_walk(SelectSmem& S, uint32_t need, int lane) {
-    uint32_t mine = 0u;
+/* A histogram walked down from its top bin by one warp: the bin where the count reaches `need`, and what is still needed in it. */
+__device__ __forceinline__ void hist_walk(ChoiceSmem& S, uint32_t need, int lane) {
+    uint32_t h[8], mine = 0u;
+    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(S.hist + 248 - 8 * lane);
+    *reinterpret_cast<uint4*>(h + 4) = *reinterpret_cast<const uint4*>(S.hist + 252 - 8 * lane);
 #pragma unroll
-    for (int b = 0; b < 8; ++b) mine += S.hist[255 - 8 * lane - b];
+    for (int b = 0; b < 8; ++b) mine += h[b];
     uint32_t upto = mine;
+#pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
     const unsigned reached = __ballot_sync(0xffffffffu, upto >= need);
     if (lane == __ffs(reached) - 1) {
-        uint32_t covered = upto - mine, bin = 255u - 8u * (uint32_t)lane;
-        while (covered + S.hist[bin] < need) covered += S.hist[bin--];
-        S.bin = bin; S.need = need - covered; S.in_bin = S.hist[bin];
+        uint32_t covered = upto - mine;
+        bool found = false;
+#pragma unroll
+        for (int b = 7; b >= 0; --b)
+            if (!found) {
+                if (covered + h[b] >= need) { found = true; S.bin = 248u - 8u * (uint32_t)lane + b; S.need = need - covered; S.in_bin = h[b]; }
+                else covered += h[b];
+            }
     }
 }
 
-/* The `take` greatest of keys[0..m) (equal keys: the lower index), their indexes ascending into out; m > take > 0.  Called by
- * SP_THREADS threads.
- * First a histogram of 256 steps of equal width between the least and the greatest finite score: the bin that the last of the
+/* The `take` greatest of keys[0..m) (equal keys: the lower index), their indexes ascending into S.picked; m > take > 0.
+ * Called by SP_THREADS threads.
+ * A histogram of 256 steps of equal width between the least and the greatest finite score: the bin that the last of the
  * chosen falls in rarely holds more than a few (a tail of scores is thin), and those few are ranked against each other.  Where
- * it holds more than SP_LIST — many equal scores — its keys are counted a byte at a time instead. */
+ * that is more than SP_LIST — many equal scores — its keys are counted a byte at a time instead, and the choice is written
+ * in order by two passes over all keys, as it is for more than SP_LIST blocks. */
 template <int SHIFT>
-__device__ __noinline__ void select_keys(const unsigned long long* keys, uint32_t m, uint32_t take, uint32_t* out, SelectSmem& S) {
+__device__ __noinline__ void choose(ChoiceSmem& S, uint32_t m, uint32_t take) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t* key_hi = reinterpret_cast<const uint32_t*>(keys) + 1;
     float mn = INFINITY, mx = -INFINITY;
     for (uint32_t i = tid; i < m; i += SP_THREADS) {
-        const float f = key_float<SHIFT>(key_hi[2 * i]);
+        const float f = key_float<SHIFT>(S.keys[i]);
         if (fabsf(f) < 3.0e38f) { mn = fminf(mn, f); mx = fmaxf(mx, f); }
     }
+#pragma unroll
     for (int x = 16; x > 0; x >>= 1) { mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, x)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x)); }
     if (lane == 0) { S.lo[warp] = mn; S.hi[warp] = mx; }
     S.hist[tid] = 0u;
-    if (tid == 0) S.n_list = 0u;
-    sp_sync();
+    if (tid == 0) { S.n_list = 0u; S.n_sure = 0u; }
+    __syncthreads();
 #pragma unroll
     for (int w = 0; w < SP_WARPS; ++w) { mn = fminf(mn, S.lo[w]); mx = fmaxf(mx, S.hi[w]); }
     if (!(mn < mx)) { mn = 0.f; mx = 0.f; }
     const float per = mx > mn ? 255.99f / (mx - mn) : 0.f;
-    auto bin_of = [&](uint32_t i) { return (uint32_t)min(max((int)((key_float<SHIFT>(key_hi[2 * i]) - mn) * per), 0), 255); };
-    for (uint32_t i = tid; i < m; i += SP_THREADS) atomicAdd(&S.hist[bin_of(i)], 1u);
-    sp_sync();
+    for (uint32_t i = tid; i < m; i += SP_THREADS) {
+        const uint32_t b = (uint32_t)min(max((int)((key_float<SHIFT>(S.keys[i]) - mn) * per), 0), 255);
+        S.bins[i] = (uint8_t)b;
+        atomicAdd(&S.hist[b], 1u);
+    }
+    __syncthreads();
     if (warp == 0) hist_walk(S, take, lane);
-    sp_sync();
+    __syncthreads();
     const uint32_t bin = S.bin, need = S.need, in_bin = S.in_bin;
-    /* keys of that bin above `cut`, and the first `ties` of those that equal it, belong to the choice */
-    if (in_bin == need) {
-        if (tid == 0) { S.cut = 0ull; S.ties = 0xFFFFFFFFu; }       /* the whole bin does (no key is 0 or less) */
-        sp_sync();
-    } else if (in_bin <= SP_LIST) {
-        for (uint32_t i = tid; i < m; i += SP_THREADS) if (bin_of(i) == bin) S.list[atomicAdd(&S.n_list, 1u)] = keys[i];
-        sp_sync();
+    if (take <= SP_LIST && in_bin <= SP_LIST) {
+        /* what lies above the bin is sure; the bin's own are listed and ranked */
+        for (uint32_t i4 = tid; i4 < (m + 3u) / 4u; i4 += SP_THREADS) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(S.bins)[i4];
+            if (__vcmpgeu4(w, bin * 0x01010101u) == 0u) continue;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t i = 4u * i4 + x, b = (w >> (8 * x)) & 255u;
+                if (i >= m || b < bin) continue;
+                if (b > bin) S.sure[atomicAdd(&S.n_sure, 1u)] = i;
+                else { const uint32_t z = atomicAdd(&S.n_list, 1u); S.list[z] = i; S.list_key[z] = S.keys[i]; }
+            }
+        }
+        __syncthreads();
         if ((uint32_t)tid < in_bin) {
-            const unsigned long long k = S.list[tid];
-            uint32_t above = 0u, upto = 0u;
-            for (uint32_t j = 0; j < in_bin; ++j) { const unsigned long long x = S.list[j]; above += x > k; upto += x >= k; }
-            if (above < need && need <= upto) { S.cut = k; S.ties = need - above; }     /* equal keys write the same */
+            const unsigned long long k = S.list_key[tid];
+            const uint32_t i = S.list[tid];
+            uint32_t ahead = 0u;
+            for (uint32_t j = 0; j < in_bin; ++j) { const unsigned long long x = S.list_key[j]; ahead += x > k || (x == k && S.list[j] < i); }
+            if (ahead < need) S.sure[take - need + ahead] = i;
         }
-        sp_sync();
-    } else {
-        unsigned long long known = 0ull, cut = 0ull;
-        uint32_t left = need;
-        for (int shift = 56; shift >= 0; shift -= 8) {
-            S.hist[tid] = 0u;
-            sp_sync();
-            for (uint32_t i = tid; i < m; i += SP_THREADS)
-                if ((keys[i] & known) == cut && bin_of(i) == bin) atomicAdd(&S.hist[(uint32_t)(keys[i] >> shift) & 255u], 1u);
-            sp_sync();
-            if (warp == 0) hist_walk(S, left, lane);
-            sp_sync();
-            cut |= (unsigned long long)S.bin << shift; left = S.need; known |= 255ull << shift;
-            sp_sync();
+        __syncthreads();
+        if ((uint32_t)tid < take) {
+            const uint32_t i = S.sure[tid];
+            uint32_t at = 0u, j = 0u;
+            for (; j + 4u <= take; j += 4u) { const uint4 x = *reinterpret_cast<const uint4*>(S.sure + j); at += (x.x < i) + (x.y < i) + (x.z < i) + (x.w < i); }
+            for (; j < take; ++j) at += S.sure[j] < i;
+            S.picked[at] = i;
         }
-        if (tid == 0) { S.cut = cut; S.ties = left; }
-        sp_sync();
+        __syncthreads();
+        return;
+    }
+    /* keys of that bin above `cut`, and the first `ties` of those that equal it, belong to the choice */
+    unsigned long long known = 0ull, cut = 0ull;
+    uint32_t ties = need;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        S.hist[tid] = 0u;
+        __syncthreads();
+        for (uint32_t i = tid; i < m; i += SP_THREADS)
+            if (S.bins[i] == bin && (S.keys[i] & known) == cut) atomicAdd(&S.hist[(uint32_t)(S.keys[i] >> shift) & 255u], 1u);
+        __syncthreads();
+        if (warp == 0) hist_walk(S, ties, lane);
+        __syncthreads();
+        cut |= (unsigned long long)S.bin << shift; ties = S.need; known |= 255ull << shift;
+        __syncthreads();
     }
     /* in index order: each warp owns a run of indexes; one pass counts, one writes */
-    const unsigned long long cut = S.cut;
-    const uint32_t ties = S.ties, run = ((m + SP_THREADS - 1) / SP_THREADS) * 32u, i0 = warp * run, i1 = min(m, i0 + run);
+    const uint32_t run = ((m + SP_THREADS - 1) / SP_THREADS) * 32u, i0 = warp * run;
     uint32_t n_in = 0u, n_tie = 0u;
     for (uint32_t i = i0 + lane; i < i0 + run; i += 32) {
         bool in = false, tie = false;
-        if (i < i1) { const uint32_t b = bin_of(i); in = b > bin || (b == bin && keys[i] > cut); tie = b == bin && keys[i] == cut; }
+        if (i < m) { const uint32_t b = S.bins[i]; in = b > bin || (b == bin && S.keys[i] > cut); tie = b == bin && S.keys[i] == cut; }
         n_in += __popc(__ballot_sync(0xffffffffu, in)); n_tie += __popc(__ballot_sync(0xffffffffu, tie));
     }
     if (lane == 0) { S.warp_in[warp] = n_in; S.warp_tie[warp] = n_tie; }
-    sp_sync();
+    __syncthreads();
     uint32_t at = 0u, tied = 0u;
 #pragma unroll
     for (int w = 0; w < SP_WARPS; ++w) if (w < warp) { at += S.warp_in[w]; tied += S.warp_tie[w]; }
@@ -206,24 +239,27 @@ __device__ __noinline__ void select_keys(const unsigned long long* keys, uint32_
     const unsigned below = (1u << lane) - 1u;
     for (uint32_t i = i0 + lane; i < i0 + run; i += 32) {
         bool in = false, tie = false;
-        if (i < i1) { const uint32_t b = bin_of(i); in = b > bin || (b == bin && keys[i] > cut); tie = b == bin && keys[i] == cut; }
+        if (i < m) { const uint32_t b = S.bins[i]; in = b > bin || (b == bin && S.keys[i] > cut); tie = b == bin && S.keys[i] == cut; }
         const unsigned tb = __ballot_sync(0xffffffffu, tie);
         in |= tie && tied + __popc(tb & below) < ties;
         const unsigned ib = __ballot_sync(0xffffffffu, in);
-        if (in) out[at + __popc(ib & below)] = i;
+        if (in) S.picked[at + __popc(ib & below)] = i;
         at += __popc(ib); tied += __popc(tb);
     }
-    sp_sync();
+    __syncthreads();
 }
 
-__device__ __forceinline__ void st_cluster_u64(const void* local, uint32_t rank, unsigned long long v) {
+__device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
-    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote), "l"(v) : "memory");
+    return remote;
 }
+__device__ __forceinline__ void st_cluster_u64(uint32_t at, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
+__device__ __forceinline__ void st_cluster_u32(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ void st_cluster_f32(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
 
 template <int D, int DT, int NHT>
-__global__ void __launch_bounds__(SP_THREADS + 32, D == 256 ? 1 : 2)
+__global__ void __launch_bounds__(SP_THREADS, D == 256 ? 1 : 2)
 paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const SparseParams P) {
     using Cfg = SparseCfg<D>;
     using E = Elem<DT>;
@@ -236,17 +272,14 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     uint8_t* smem = (uint8_t*)(((uintptr_t)sp_raw + 1023) & ~(uintptr_t)1023);
     const uint32_t keep = P.first + P.last + P.top;
     uint8_t* ring = smem;
+    ChoiceSmem& S = *(ChoiceSmem*)ring;
     uint8_t* q_base = ring + Cfg::STAGES * Cfg::STAGE_BYTES;
-    uint64_t* full = (uint64_t*)(q_base + Q_BYTES);
+    float* meet = (float*)(q_base + Q_BYTES);                     /* [CL][HPB][D / CL] partials of this block's columns, from every peer */
+    float* meet_ml = meet + HPB * D;                              /* [16][HPB][2] */
+    uint64_t* full = (uint64_t*)(meet_ml + 16 * HPB * 2);
     uint64_t* empty = full + Cfg::STAGES;
     volatile uint32_t* abort_flag = (volatile uint32_t*)(empty + Cfg::STAGES);
-    int32_t* slots = (int32_t*)(empty + Cfg::STAGES + 1);                         /* [keep] the chosen blocks' places in the pool */
-    uint32_t* ids = (uint32_t*)(slots + keep);                                    /* [top] the chosen blocks' numbers */
-    uint32_t* picked = ids + P.top;                                               /* [top] */
-    /* before the first tile the ring holds the scores */
-    unsigned long long* keys = (unsigned long long*)ring;                         /* [SP_CHUNK + top] */
-    double* qsum = (double*)(keys + SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX);     /* [D] */
-    SelectSmem& S = *(SelectSmem*)(qsum + D);
+    int32_t* slots = (int32_t*)(empty + Cfg::STAGES + 1);         /* [keep] the chosen blocks' places in the pool */
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t CL = cluster_nctarank(), crank = cluster_ctarank();
@@ -263,6 +296,21 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     asm volatile("griddepcontrol.wait;" ::: "memory");      /* everything read below may be the work of the grid ahead */
 
     const int32_t seq = P.row_seq[r], pos = P.row_pos[r];
+    /* the query does not hang on them: asked for at the same time */
+    constexpr int QV = (HPB * (D / 8) + SP_THREADS - 1) / SP_THREADS;
+    const uint16_t* qrow = P.q + (size_t)r * P.q_stride;
+    uint4 qv[QV];
+    double qs = 0;
+#pragma unroll
+    for (int x = 0; x < QV; ++x) {
+        const uint32_t i = tid + x * SP_THREADS, h = i / (D / 8);
+        qv[x] = h < heads ? *reinterpret_cast<const uint4*>(qrow + (size_t)(head0 + h) * D + (i % (D / 8)) * 8) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (P.top && tid < D) {
+        const uint16_t* src = qrow + (size_t)kvh * P.group * D + tid;
+#pragma unroll 8
+        for (uint32_t h = 0; h < P.group; ++h) qs += (double)E::to_float(src[h * D]);
+    }
     if (seq < 0 || (uint32_t)seq >= P.seqs) { if (seq >= 0 && tid == 0 && crank == 0 && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE); return; }
     const size_t out0 = (size_t)r * P.q_heads + head0;
     int32_t* chosen = P.chosen && hb == 0 && crank == 0 ? P.chosen + ((size_t)r * P.kv_heads + kvh) * keep : nullptr;
@@ -277,145 +325,166 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     }
     const PagedChoice c = paged_choice((uint32_t)pos, P.block, P.first, P.last, P.top);
     const int32_t* row = P.table + (size_t)seq * P.stride;
-    const uint16_t* qrow = P.q + (size_t)r * P.q_stride;
     bool bad = false;
+    /* a block whose page is none is asked for past the pool's last row, where TMA answers zeros */
+    auto slot_of = [&](int32_t place) { return place < 0 ? (int32_t)(P.pool_pages * P.page_pos) : (int32_t)((uint32_t)place * P.block); };
 
     /* a peer's shared memory may be written only once the peer runs: arrive now, wait ahead of the first score */
     if (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    if (warp < NW) {
-        for (int i = tid; i < HPB * (D / 8); i += SP_THREADS) {
-            const int h = i / (D / 8), j = i % (D / 8);
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if ((uint32_t)h < heads) x = *reinterpret_cast<const uint4*>(qrow + (size_t)(head0 + h) * D + j * 8);
-            *reinterpret_cast<uint4*>(q_base + (j / 8) * (HPB * 128) + swz128(h, j % 8)) = x;
+
+    /* Means are dealt to the cluster's warps BPS at a time, U times round: mean `i` of this lane's u-th is
+     * i0 + u * STRIDE + (its warp's place) * BPS + lane / LPB.  Lane l looks up the page of the (l / BPS)-th round's l % BPS-th. */
+    const uint32_t STRIDE = CL * NW * Cfg::BPS, w_at = (crank * NW + warp) * Cfg::BPS;
+    auto look_up = [&](uint32_t base, uint32_t n, uint32_t i0) {
+        const uint32_t i = i0 + (lane / Cfg::BPS) * STRIDE + w_at + lane % Cfg::BPS;
+        if (lane >= Cfg::WB || i >= n) return -1;
+        const int32_t at = paged_block(row, P.stride, P.pool_pages, P.per, base + i);
+        bad |= at < 0;
+        return at;
+    };
+    uint4 x[Cfg::U][Cfg::CPL];
+    auto load = [&](int32_t mine) {
+#pragma unroll
+        for (int u = 0; u < Cfg::U; ++u) {
+            const int32_t at = __shfl_sync(0xffffffffu, mine, u * Cfg::BPS + lane / Cfg::LPB);
+            const uint4* src = reinterpret_cast<const uint4*>(P.means + ((size_t)max(at, 0) * P.kv_heads + kvh) * D) + lane % Cfg::LPB;
+#pragma unroll
+            for (int y = 0; y < Cfg::CPL; ++y) x[u][y] = at >= 0 ? __ldg(src + y * Cfg::LPB) : make_uint4(0u, 0u, 0u, 0u);
         }
-        if (c.take)
-            for (int e = tid; e < D; e += SP_THREADS) {
-                double s = 0;
-                for (uint32_t h = 0; h < P.group; ++h) s += (double)E::to_float(qrow[(size_t)(kvh * P.group + h) * D + e]);
-                qsum[e] = s * W::up();
-            }
+    };
+    int32_t mine = -1, next = -1;
+    if (c.take) {
+        mine = look_up(c.lo, min(SP_CHUNK, c.hi - c.lo), 0u);
+        load(mine);
+    }
+#pragma unroll
+    for (int z = 0; z < QV; ++z) {
+        const uint32_t i = tid + z * SP_THREADS, h = i / (D / 8), j = i % (D / 8);
+        if (h < HPB) *reinterpret_cast<uint4*>(q_base + (j / 8) * (HPB * 128) + swz128(h, j % 8)) = qv[z];
+    }
+    /* the summed query in pairs, a round's pairs side by side for the lanes that share a mean */
+    if (P.top && tid < D) S.qsum[((((tid / 8) / Cfg::LPB) * 4 + (tid % 8) / 2) * Cfg::LPB + (tid / 8) % Cfg::LPB) * 2 + tid % 2] = qs * W::up();
+    /* the blocks that are always attended, while the means are on their way */
+    for (uint32_t i = tid; i < keep; i += SP_THREADS) {
+        if (i >= c.lo && i < c.lo + c.take) continue;
+        int32_t id = -1;
+        if (i < c.count) {
+            id = i < c.lo ? (int32_t)i : (int32_t)(c.hi + (i - c.lo - c.take));
+            const int32_t at = paged_block(row, P.stride, P.pool_pages, P.per, (uint32_t)id);
+            bad |= at < 0;
+            slots[i] = slot_of(at);
+        }
+        if (chosen) chosen[i] = id;
     }
     __syncthreads();
     if (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     /* ---- scores and choice, a chunk of blocks at a time ---- */
-    uint32_t have = 0;                                                    /* the best of the chunks so far: keys[0..have), ids[0..have) */
+    uint32_t have = 0;                                                    /* the best of the chunks so far: keys, place, ids [0..have) */
     for (uint32_t base = c.lo; c.take && base < c.hi; base += SP_CHUNK) {
         const uint32_t n = min(SP_CHUNK, c.hi - base);
-        if (warp < NW) {
-            double qd[Cfg::CPL][8];
-#pragma unroll
-            for (int x = 0; x < Cfg::CPL; ++x)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) qd[x][e] = qsum[(x * Cfg::LPB + lane % Cfg::LPB) * 8 + e];
-            const uint32_t step = CL * NW * Cfg::WB;
-            const uint32_t i_lane = (crank * NW + warp) * Cfg::WB + lane;             /* the mean whose place lane `lane` looks up */
-            auto place = [&](uint32_t i) {
-                if (lane >= Cfg::WB || i >= n) return -1;
-                const int32_t s = paged_block_slot(row, P.stride, P.pool_pages, P.page_pos, P.block, base + i);
-                if (s < 0) { bad = true; return -1; }
-                return (int32_t)((uint32_t)s / P.block);
-            };
-            int32_t mine = place(i_lane);
-            for (uint32_t i0 = i_lane - lane; i0 < n; i0 += step) {
-                uint4 x[Cfg::U][Cfg::CPL];
-                bool there[Cfg::U];
-#pragma unroll
-                for (int u = 0; u < Cfg::U; ++u) {
-                    const int32_t m = __shfl_sync(0xffffffffu, mine, u * Cfg::BPS + lane / Cfg::LPB);
-                    there[u] = m >= 0;
-                    const uint4* src = reinterpret_cast<const uint4*>(P.means + ((size_t)(there[u] ? m : 0) * P.kv_heads + kvh) * D) + lane % Cfg::LPB;
-#pragma unroll
-                    for (int y = 0; y < Cfg::CPL; ++y) x[u][y] = there[u] ? __ldg(src + y * Cfg::LPB) : make_uint4(0u, 0u, 0u, 0u);
-                }
-                mine = place(i0 + step + lane);
+        {
+            if (base != c.lo) { mine = look_up(base, n, 0u); load(mine); }
+            for (uint32_t i0 = 0; i0 < n; i0 += STRIDE * Cfg::U) {
+                next = look_up(base, n, i0 + STRIDE * Cfg::U);
                 double s[Cfg::U];
 #pragma unroll
-                for (int u = 0; u < Cfg::U; ++u) {
-                    double a = 0;
+                for (int g = 0; g < Cfg::U; g += 4) {
+                    s[g] = s[g + 1] = s[g + 2] = s[g + 3] = 0;
+                    if (i0 + g * STRIDE + w_at >= n) continue;
                     uint32_t special = 0u;
 #pragma unroll
-                    for (int y = 0; y < Cfg::CPL; ++y) {
-                        const uint32_t w[4] = {x[u][y].x, x[u][y].y, x[u][y].z, x[u][y].w};
+                    for (int y = 0; y < Cfg::CPL; ++y)
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            a = fma(W::lo(w[z]), qd[y][2 * z], a); a = fma(W::hi(w[z]), qd[y][2 * z + 1], a);
-                            special = __vmaxu2(special, w[z] & 0x7FFF7FFFu);
+                            const double2 q2 = *reinterpret_cast<const double2*>(S.qsum + ((y * 4 + z) * Cfg::LPB + lane % Cfg::LPB) * 2);
+#pragma unroll
+                            for (int u = g; u < g + 4; ++u) {
+                                const uint32_t w = z == 0 ? x[u][y].x : z == 1 ? x[u][y].y : z == 2 ? x[u][y].z : x[u][y].w;
+                                s[u] = fma(W::lo(w), q2.x, s[u]); s[u] = fma(W::hi(w), q2.y, s[u]);
+                                special = __vmaxu2(special, w & 0x7FFF7FFFu);
+                            }
                         }
-                    }
                     if ((special & 0xFFFFu) >= W::SPECIAL || (special >> 16) >= W::SPECIAL) {
-                        a = 0;
 #pragma unroll
-                        for (int y = 0; y < Cfg::CPL; ++y) {
-                            const uint32_t w[4] = {x[u][y].x, x[u][y].y, x[u][y].z, x[u][y].w};
+                        for (int u = g; u < g + 4; ++u) {
+                            double a = 0;
+                            bool is = false;
 #pragma unroll
-                            for (int z = 0; z < 4; ++z) { const float2 f = E::unpack2(w[z]); a += (double)f.x * qd[y][2 * z]; a += (double)f.y * qd[y][2 * z + 1]; }
+                            for (int y = 0; y < Cfg::CPL; ++y)
+#pragma unroll
+                                for (int z = 0; z < 4; ++z) {
+                                    const uint32_t w = z == 0 ? x[u][y].x : z == 1 ? x[u][y].y : z == 2 ? x[u][y].z : x[u][y].w;
+                                    const float2 f = E::unpack2(w);
+                                    const double2 q2 = *reinterpret_cast<const double2*>(S.qsum + ((y * 4 + z) * Cfg::LPB + lane % Cfg::LPB) * 2);
+                                    a += (double)f.x * q2.x; a += (double)f.y * q2.y;
+                                    is |= (w & 0x7FFFu) >= W::SPECIAL || ((w >> 16) & 0x7FFFu) >= W::SPECIAL;
+                                }
+                            if (is) s[u] = a;
                         }
                     }
-                    s[u] = a;
                 }
-                /* the lanes' parts of four means at once: each exchange halves what a lane still holds; whichever of two lanes adds,
-                 * the sum is the same */
-                constexpr int T0 = Cfg::LPB / 2, T1 = Cfg::LPB / 4;
-                const bool up0 = (lane & T0) != 0, up1 = (lane & T1) != 0;
-                double a0 = up0 ? s[2] : s[0], a1 = up0 ? s[3] : s[1];
-                a0 += __shfl_xor_sync(0xffffffffu, up0 ? s[0] : s[2], T0);
-                a1 += __shfl_xor_sync(0xffffffffu, up0 ? s[1] : s[3], T0);
-                double v = up1 ? a1 : a0;
-                v += __shfl_xor_sync(0xffffffffu, up1 ? a0 : a1, T1);
+                const int32_t old = mine;
+                mine = next;
+                if (i0 + STRIDE * Cfg::U < n) load(mine);
+                /* the lanes' parts of eight means at once: each exchange halves what a lane still holds; whichever of two lanes
+                 * adds, the sum is the same */
+                constexpr int T0 = Cfg::LPB / 2, T1 = Cfg::LPB / 4, T2 = Cfg::LPB / 8;
+                const bool up0 = (lane & T0) != 0, up1 = (lane & T1) != 0, up2 = (lane & T2) != 0;
+                double a[4], b[2];
 #pragma unroll
-                for (int t = T1 / 2; t > 0; t >>= 1) v += __shfl_xor_sync(0xffffffffu, v, t);
-                const int u = (up0 ? 2 : 0) + (up1 ? 1 : 0);
-                const uint32_t i = i0 + u * Cfg::BPS + lane / Cfg::LPB;
-                bool is = false;
+                for (int u = 0; u < 4; ++u) a[u] = (up0 ? s[4 + u] : s[u]) + __shfl_xor_sync(0xffffffffu, up0 ? s[u] : s[4 + u], T0);
 #pragma unroll
-                for (int z = 0; z < Cfg::U; ++z) is = z == u ? there[z] : is;
+                for (int u = 0; u < 2; ++u) b[u] = (up1 ? a[2 + u] : a[u]) + __shfl_xor_sync(0xffffffffu, up1 ? a[u] : a[2 + u], T1);
+                double v = (up2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, up2 ? b[0] : b[1], T2);
+                if (T2 == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
+                const int u = (up0 ? 4 : 0) + (up1 ? 2 : 0) + (up2 ? 1 : 0);
+                const int32_t at = __shfl_sync(0xffffffffu, old, u * Cfg::BPS + lane / Cfg::LPB);
+                const uint32_t i = i0 + u * STRIDE + w_at + lane / Cfg::LPB;
                 if (i < n) {
-                    const unsigned long long k = score_key(is ? v : -INFINITY);
-                    if (CL == 1) { if (lane % T1 == 0) keys[have + i] = k; }
-                    else for (uint32_t to = lane % T1; to < CL; to += T1) st_cluster_u64(&keys[have + i], to, k);
+                    const unsigned long long k = score_key(at >= 0 ? v : -INFINITY);
+                    if (CL == 1) { if (lane % T2 == 0) { S.keys[have + i] = k; S.place[have + i] = at; } }
+                    else for (uint32_t to = lane % T2; to < CL; to += T2) { st_cluster_u64(peer_addr(&S.keys[have + i], to), k); st_cluster_u32(peer_addr(&S.place[have + i], to), (uint32_t)at); }
                 }
             }
         }
         if (CL > 1) cluster_sync_all(); else __syncthreads();
         const uint32_t m = have + n;
         const bool more = base + SP_CHUNK < c.hi;
-        if (warp < NW) {
+        {
             if (m <= c.take) {
-                for (uint32_t i = tid; i < n; i += SP_THREADS) ids[have + i] = base + i;
+                for (uint32_t i = tid; i < n; i += SP_THREADS) S.ids[have + i] = base + i;
             } else {
-                select_keys<W::SHIFT>(keys, m, c.take, picked, S);
-                /* the chosen move to the front, in order: read all, then write */
-                unsigned long long kk[SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS];
-                uint32_t ii[SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS];
+                choose<W::SHIFT>(S, m, c.take);
+                auto id_of = [&](uint32_t i) { return i < have ? S.ids[i] : base + (i - have); };
+                if (more) {
+                    /* the chosen move to the front, in order: read all, then write */
+                    constexpr int KP = SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS;
+                    unsigned long long kk[KP];
+                    uint32_t ii[KP];
+                    int32_t pp[KP];
 #pragma unroll
-                for (int z = 0; z < (int)(SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS); ++z) {
-                    const uint32_t i = tid + z * SP_THREADS;
-                    if (i < c.take) { const uint32_t at = picked[i]; kk[z] = keys[at]; ii[z] = at < have ? ids[at] : base + (at - have); }
-                }
-                sp_sync();
+                    for (int z = 0; z < KP; ++z) {
+                        const uint32_t i = tid + z * SP_THREADS;
+                        if (i < c.take) { const uint32_t at = S.picked[i]; kk[z] = S.keys[at]; ii[z] = id_of(at); pp[z] = S.place[at]; }
+                    }
+                    __syncthreads();
 #pragma unroll
-                for (int z = 0; z < (int)(SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS); ++z) {
-                    const uint32_t i = tid + z * SP_THREADS;
-                    if (i < c.take) { keys[i] = kk[z]; ids[i] = ii[z]; }
+                    for (int z = 0; z < KP; ++z) {
+                        const uint32_t i = tid + z * SP_THREADS;
+                        if (i < c.take) { S.keys[i] = kk[z]; S.ids[i] = ii[z]; S.place[i] = pp[z]; }
+                    }
+                } else {
+                    for (uint32_t i = tid; i < c.take; i += SP_THREADS) {
+                        const uint32_t at = S.picked[i];
+                        slots[c.lo + i] = slot_of(S.place[at]);
+                        if (chosen) chosen[c.lo + i] = (int32_t)id_of(at);
+                    }
                 }
             }
         }
         have = min(m, c.take);
         if (more) { if (CL > 1) cluster_sync_all(); else __syncthreads(); }       /* no one writes the next scores over what a peer still reads */
-    }
-    __syncthreads();
-    for (uint32_t i = tid; i < keep; i += blockDim.x) {
-        int32_t id = -1;
-        if (i < c.count) {
-            id = i < c.lo ? (int32_t)i : i < c.lo + c.take ? (int32_t)ids[i - c.lo] : (int32_t)(c.hi + (i - c.lo - c.take));
-            const int32_t slot = paged_block_slot(row, P.stride, P.pool_pages, P.page_pos, P.block, (uint32_t)id);
-            bad |= slot < 0;
-            /* a block whose page is none is asked for past the pool's last row, where TMA answers zeros */
-            slots[i] = slot < 0 ? (int32_t)(P.pool_pages * P.page_pos) : slot;
-        }
-        if (chosen) chosen[i] = id;
     }
     fence_proxy_async_smem();            /* the scores' accesses to the ring come before the loads into it */
     __syncthreads();
@@ -432,28 +501,27 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
         for (int k = 0; k < VS; ++k) { oacc[n][k][0] = oacc[n][k][1] = oacc[n][k][2] = oacc[n][k][3] = 0.f; }
     }
-    if (warp == NW) {
-        /* ---- the loads: one box of 64 columns by min(B, 64) positions a lane ---- */
-        const uint32_t br = min(P.block, 64u), sub = 64u / br;
-        const uint64_t pol = l2_policy_evict_first();
-        for (int it = 0; it < nt; ++it) {
-            const int s = it % Cfg::STAGES;
-            if (it >= Cfg::STAGES && !mbar_wait(&empty[s], ((it / Cfg::STAGES) - 1) & 1, abort_flag, P.status)) break;
-            const uint32_t p0 = (crank + it * CL) * 64u;
-            const uint32_t boxes = min(sub, (live - p0 + br - 1u) / br);
-            uint8_t* st = ring + s * Cfg::STAGE_BYTES;
-            if (lane == 0) mbar_expect_tx(&full[s], boxes * br * 128u * Cfg::BOXES * 2u);
-            __syncwarp();
-            for (uint32_t i = lane; i < boxes * Cfg::BOXES * 2u; i += 32) {
-                const uint32_t b = i / (Cfg::BOXES * 2u), x = i % (Cfg::BOXES * 2u), col = x % Cfg::BOXES;
-                const uint32_t at = p0 + b * br;
-                const int32_t y = slots[at / P.block] + (int32_t)(at % P.block);
-                tma_load_2d_hint(st + (x / Cfg::BOXES) * Cfg::K_BYTES + col * Cfg::BOX_BYTES + b * br * 128u, x < Cfg::BOXES ? (const void*)&kmap : (const void*)&vmap, &full[s],
-                                 (int32_t)(kvh * D + col * 64u), y, pol);
-            }
-            __syncwarp();
+    /* the loads of tile `it`: one box of 64 columns by min(B, 64) positions a lane of one warp */
+    const uint32_t br = min(P.block, 64u), sub = 64u / br;
+    const uint64_t pol = l2_policy_evict_first();
+    auto fetch = [&](int it) {
+        const int s = it % Cfg::STAGES;
+        const uint32_t p0 = (crank + it * CL) * 64u;
+        const uint32_t boxes = min(sub, (live - p0 + br - 1u) / br);
+        uint8_t* st = ring + s * Cfg::STAGE_BYTES;
+        if (lane == 0) mbar_expect_tx(&full[s], boxes * br * 128u * Cfg::BOXES * 2u);
+        __syncwarp();
+        for (uint32_t i = lane; i < boxes * Cfg::BOXES * 2u; i += 32) {
+            const uint32_t b = i / (Cfg::BOXES * 2u), x = i % (Cfg::BOXES * 2u), col = x % Cfg::BOXES;
+            const uint32_t at = p0 + b * br;
+            const int32_t y = slots[at / P.block] + (int32_t)(at % P.block);
+            tma_load_2d_hint(st + (x / Cfg::BOXES) * Cfg::K_BYTES + col * Cfg::BOX_BYTES + b * br * 128u, x < Cfg::BOXES ? (const void*)&kmap : (const void*)&vmap, &full[s],
+                             (int32_t)(kvh * D + col * 64u), y, pol);
         }
-    } else {
+        __syncwarp();
+    };
+    if (warp < Cfg::STAGES && warp < nt) fetch(warp);
+    {
         const uint32_t q_u32 = smem_u32(q_base);
         auto load_qfrag = [&](int n, int kk, uint32_t& b0, uint32_t& b1) {
             /* B fragment of Q^T for heads n*8..n*8+7, columns kk*16..+15: two 8x8 blocks (chunks 2kk, 2kk+1) */
@@ -469,6 +537,11 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         const int r_lo = lane >> 2, w4 = warp & 3, half = warp >> 2;      /* positions [16 w4, +16) of a tile, value columns [half D/2, +D/2) */
         for (int it = 0; it < nt; ++it) {
             const int s = it % Cfg::STAGES;
+            /* the warps take turns to ask for the tile that goes where the one before this lay, once all have left it */
+            if (it > 0 && it - 1 + Cfg::STAGES < nt && warp == it % NW) {
+                if (!mbar_wait(&empty[(it - 1) % Cfg::STAGES], ((it - 1) / Cfg::STAGES) & 1, abort_flag, P.status)) break;
+                fetch(it - 1 + Cfg::STAGES);
+            }
             if (!mbar_wait(&full[s], (it / Cfg::STAGES) & 1, abort_flag, P.status)) break;
             uint8_t* stage = ring + s * Cfg::STAGE_BYTES;
             const uint32_t kst = smem_u32(stage), vst = kst + Cfg::K_BYTES;
@@ -573,10 +646,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     float* wm = (float*)ring;                         /* [PW][HPB] */
     float* wl = wm + PW * HPB;                        /* [PW][HPB] */
     float* wo = wl + PW * HPB;                        /* [PW][HPB][D] */
-    float* bacc = wo + (size_t)PW * HPB * D;          /* [HPB][D] */
-    float* bm = bacc + HPB * D;                       /* [HPB] log2 units */
-    float* bl = bm + HPB;                             /* [HPB] */
-    if (warp < NW) {
+    {
         const int r_lo = lane >> 2, c2 = (lane & 3) * 2, w4 = warp & 3, half = warp >> 2;
 #pragma unroll
         for (int n = 0; n < NHT; ++n) {
@@ -614,28 +684,27 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             if (mw != -INFINITY) { const float f = fast_exp2(mw - m); acc += wo[(size_t)(w * HPB + h) * D + e] * f; l += wl[w * HPB + h] * f; }
         }
         if (CL == 1) answer(h, e, m, l, acc);
-        else { bacc[i] = acc; if (e == 0) { bm[h] = m; bl[h] = l; } }
+        else {
+            /* columns [c D/CL, (c+1) D/CL) of every head meet in thread block c */
+            const uint32_t DS = D / CL, to = e / DS;
+            st_cluster_f32(peer_addr(meet + (crank * HPB + h) * DS + e % DS, to), acc);
+            if (e % DS == 0) { st_cluster_f32(peer_addr(meet_ml + (crank * HPB + h) * 2, to), m); st_cluster_f32(peer_addr(meet_ml + (crank * HPB + h) * 2 + 1, to), l); }
+        }
     }
     if (CL > 1) {
-        cluster_sync_all();
-        /* thread block c folds columns [c D/CL, (c+1) D/CL) of every head over all, in order */
+        cluster_sync_all();                           /* nothing is sent to a peer after this */
         const uint32_t DS = D / CL;
         for (uint32_t i = tid; i < heads * DS; i += blockDim.x) {
-            const uint32_t h = i / DS, e = crank * DS + i % DS;
-            float pm[16], pl[16], pa[16];
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-                if (x < (int)CL) { pm[x] = ld_cluster_f32(bm + h, x); pl[x] = ld_cluster_f32(bl + h, x); pa[x] = ld_cluster_f32(bacc + h * D + e, x); }
+            const uint32_t h = i / DS, e = i % DS;
             float m = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) if (x < (int)CL) m = fmaxf(m, pm[x]);
+            for (uint32_t x = 0; x < CL; ++x) m = fmaxf(m, meet_ml[(x * HPB + h) * 2]);
             float acc = 0.f, l = 0.f;
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-                if (x < (int)CL && pm[x] != -INFINITY) { const float f = fast_exp2(pm[x] - m); acc += pa[x] * f; l += pl[x] * f; }
-            answer(h, e, m, l, acc);
+            for (uint32_t x = 0; x < CL; ++x) {
+                const float mx = meet_ml[(x * HPB + h) * 2], f = mx == -INFINITY ? 0.f : fast_exp2(mx - m);
+                acc += meet[(x * HPB + h) * DS + e] * f; l += meet_ml[(x * HPB + h) * 2 + 1] * f;
+            }
+            answer(h, crank * DS + e, m, l, acc);
         }
-        cluster_sync_all();                           /* a peer's shared memory is there until all have read it */
     }
     if (hit && P.over) atomicOr(P.over, SV_FAULT_OVERFLOW);
     if (bad && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE);
@@ -645,14 +714,15 @@ template <int D, int DT, int NHT>
 static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& vm, const SparseParams& P, uint64_t units, uint32_t cluster, cudaStream_t st) {
     using Cfg = SparseCfg<D>;
     const uint32_t keep = P.first + P.last + P.top;
-    const size_t fixed = 1024 + (size_t)Cfg::STAGES * Cfg::STAGE_BYTES + Cfg::BOXES * 8 * NHT * 128 + (2 * Cfg::STAGES + 1) * 8;
-    const size_t smem = fixed + ((size_t)keep + 2 * P.top) * 4;
-    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX) * 8 + D * 8 + sizeof(SelectSmem), "the scores fit the ring");
-    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (size_t)(SP_WARPS / 2 + 1) * 8 * NHT * (D + 2) * 4, "the partials fit the ring");
+    constexpr size_t fixed = 1024 + (size_t)Cfg::STAGES * Cfg::STAGE_BYTES + Cfg::BOXES * 8 * NHT * 128 + 8 * NHT * (D + 32) * 4 + (2 * Cfg::STAGES + 1) * 8;
+    const size_t smem = fixed + (size_t)keep * 4;
+    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= sizeof(ChoiceSmem), "the scores fit the ring");
+    static_assert(fixed + SILVANN_B200_PAGED_KEEP_MAX * 4 <= 227 * 1024, "a thread block's shared memory");
+    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (size_t)(SP_WARPS / 2) * 8 * NHT * (D + 2) * 4, "the partials fit the ring");
     static std::atomic<bool> attr_set[SPARSE_DEVICES];
     int d = 0; cudaGetDevice(&d);
     if (d >= 0 && d < SPARSE_DEVICES && !attr_set[d].load(std::memory_order_acquire)) {
-        cudaError_t e = cudaFuncSetAttribute(paged_sparse_kernel<D, DT, NHT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + 3 * SILVANN_B200_PAGED_KEEP_MAX * 4));
+        cudaError_t e = cudaFuncSetAttribute(paged_sparse_kernel<D, DT, NHT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + SILVANN_B200_PAGED_KEEP_MAX * 4));
         if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_sparse_kernel<D, DT, NHT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         attr_set[d].store(true, std::memory_order_release);
@@ -660,7 +730,7 @@ static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& v
     cudaError_t e = cudaErrorInvalidValue;
     for (; cluster > 0; cluster /= 2) {               /* a cluster that the card cannot place goes out again half as large */
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(units * cluster)); cfg.blockDim = dim3(SP_THREADS + 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+        cfg.gridDim = dim3((unsigned)(units * cluster)); cfg.blockDim = dim3(SP_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
         cudaLaunchAttribute at[2];
         unsigned na = 0;
         if (cluster > 1u) { at[na].id = cudaLaunchAttributeClusterDimension; at[na].val.clusterDim.x = cluster; at[na].val.clusterDim.y = 1; at[na].val.clusterDim.z = 1; ++na; }
@@ -723,7 +793,7 @@ SV_EXPORT int silvann_b200_paged_sparse(void* o, float* res, int32_t* chosen, co
     memset(&P, 0, sizeof P);
     P.o = o; P.res = res; P.chosen = chosen; P.q = (const uint16_t*)q; P.means = (const uint16_t*)k_means;
     P.row_seq = row_seq; P.row_pos = row_pos; P.table = page_table; P.over = over; P.status = sv::device_status_word(); P.q_stride = q_stride; P.seqs = seqs;
-    P.stride = table_stride; P.pool_pages = (uint32_t)pool_pages; P.page_pos = page_positions; P.block = block_positions; P.q_heads = q_heads; P.kv_heads = kv_heads;
+    P.stride = table_stride; P.pool_pages = (uint32_t)pool_pages; P.page_pos = page_positions; P.block = block_positions; P.per = sv::paged_div(page_positions / block_positions); P.q_heads = q_heads; P.kv_heads = kv_heads;
     P.group = q_heads / kv_heads; P.first = first; P.last = last; P.top = top; P.scale_log2 = (1.0f / sqrtf((float)head_dim)) * SV_LOG2E;
     cudaError_t e = sv::sparse_launch(P, k_pool, v_pool, rows, head_dim, dtype, (cudaStream_t)stream);
     if (e == cudaSuccess) return SILVANN_B200_OK;

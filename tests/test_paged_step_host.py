@@ -70,17 +70,26 @@ int main() {
             const uint32_t P = B * per, pool = 7;
             for (uint32_t stride : {1u, 4u, 9u})
                 for (uint32_t b = 0; b < 60; ++b) {
-                    const int32_t got = sv::paged_block_slot(entries, stride, pool, P, B, b);
+                    const int32_t at = sv::paged_block(entries, stride, pool, sv::paged_div(per), b);
+                    const long got = at < 0 ? -1 : (long)at * B;
                     const uint32_t col = b * B / P;
                     const bool good = col < stride && entries[col] >= 0 && entries[col] < (int32_t)pool;
                     const long want = good ? (long)entries[col] * P + (long)b * B % P : -1;
-                    if (got != want || (got >= 0 && got + B > pool * P)) { printf("B %u P %u stride %u block %u: %d, not %ld\n", B, P, stride, b, got, want); return 1; }
+                    if (got != want || (got >= 0 && got + B > pool * P)) { printf("B %u P %u stride %u block %u: %ld, not %ld\n", B, P, stride, b, got, want); return 1; }
                 }
         }
     // a block far along a long table, where the column alone needs 27 bits, and the last block of the largest pool
-    if (sv::paged_block_slot(entries, 4, 7, 16, 16, 0x7FFFFFFFu / 16) != -1) return 2;
+    if (sv::paged_block(entries, 4, 7, sv::paged_div(1), 0x7FFFFFFFu / 16) != -1) return 2;
     const int32_t last[] = {(1 << 27) - 2};
-    if (sv::paged_block_slot(last, 1, (1u << 27) - 1, 16, 16, 0) != (int32_t)(((1u << 27) - 2) * 16u)) return 3;
+    if (sv::paged_block(last, 1, (1u << 27) - 1, sv::paged_div(1), 0) != (1 << 27) - 2) return 3;
+    for (uint32_t d : {1u, 2u, 3u, 5u, 7u, 48u, 64u, 641u, 65535u, 65536u, 1000003u, 0x3FFFFFFFu, 0x40000000u, 0x40000001u, 0x7FFFFFFFu}) {
+        const sv::PagedDiv x = sv::paged_div(d);
+        for (uint64_t k = 0; k < 4000; ++k)
+            for (int64_t j = -2; j <= 2; ++j) {
+                const int64_t n = (k < 2000 ? (int64_t)(k * d) : (int64_t)(0x7FFFFFFF - (k - 2000) * 1000003)) + j;
+                if (n >= 0 && n <= 0x7FFFFFFF && sv::paged_quot((uint32_t)n, x) != (uint32_t)n / d) { printf("%ld / %u\n", (long)n, d); return 6; }
+            }
+    }
     for (uint32_t p = 0; p < 3000; ++p)
         for (uint32_t B : {16u, 64u, 128u})
             for (uint32_t first : {0u, 1u, 3u}) for (uint32_t last_ : {1u, 2u}) for (uint32_t top : {0u, 1u, 7u}) {
