@@ -10,8 +10,8 @@
  *   choice  — each thread block picks the same `top` blocks from the whole list, so nothing has to be sent round again.
  *   attend  — the chosen blocks, in order, are a short cache of their own: 64-position tiles of it are dealt to the thread
  *             blocks, arrive by TMA (128-byte swizzle) in a ring, and meet an online softmax with heads as the N dimension
- *             of the warp MMAs (S^T = K Q^T, O^T = V^T P^T).  Four warps share a tile by positions, and two such sets share it
- *             by value columns (both form the scores, which is cheaper than a second set of accumulators).  The partials
+ *             of the warp MMAs (S^T = K Q^T, O^T = V^T P^T).  Some warps share a tile by positions, and their sets share it by value
+ *             columns (each set forms the scores, which is cheaper than more accumulators).  The partials
  *             meet through the cluster's shared memory, in a fixed order.  No scratch in global memory: calls share nothing.
  *
  * Why 64 bits for the scores: which block is chosen hangs on two scores next to each other, and a choice that went by the
@@ -37,16 +37,18 @@ static constexpr int SPARSE_DEVICES = 64;
 #define SP_WARPS 8
 #define SP_THREADS (SP_WARPS * 32)
 #define SP_CHUNK 4096u                        /* scores looked at in one go; the best of the chunks before them ride along */
-#define SP_CAP (SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX)
-#define SP_LIST 256u                          /* one thread each */
+#define SP_CAP (SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX + 8u)
+#define SP_LIST (2u * SP_THREADS)             /* candidates among which the border is looked for: two a thread */
 
 template <int D> struct SparseCfg {
+    static constexpr int TP = D == 256 ? 32 : 64;         /* positions a tile: 16 or 32 KB of K and V */
+    static constexpr int PW = TP / 16;                    /* warps that share a tile by positions; SP_WARPS / PW share it by value columns */
     static constexpr int BOXES = D / 64;                  /* 64-column (128-byte) boxes a row */
-    static constexpr int BOX_BYTES = 64 * 128;            /* 64 positions */
+    static constexpr int BOX_BYTES = TP * 128;
     static constexpr int K_BYTES = BOXES * BOX_BYTES;
     static constexpr int STAGE_BYTES = 2 * K_BYTES;       /* K then V */
-    static constexpr int STAGES = D == 64 ? 6 : 3;        /* 96 KB at head_dim 64 and 128 (two thread blocks an SM), 192 KB at 256 */
-    /* scores: lanes a mean, 16-byte pieces of it a lane, means a warp takes at a time */
+    static constexpr int STAGES = D == 64 ? 6 : 3;        /* 96 KB: two thread blocks an SM */
+    /* scores: lanes a mean, 16-byte pieces of it a lane, means a warp takes in a round, rounds asked for at once */
     static constexpr int LPB = D == 256 ? 16 : 8;
     static constexpr int CPL = D / 8 / LPB;
     static constexpr int BPS = 32 / LPB;
@@ -65,12 +67,13 @@ struct SparseParams {
     PagedDiv per;                       /* blocks a page */
     uint32_t seqs, stride, pool_pages, page_pos, block, q_heads, kv_heads, group, head_blocks, first, last, top;
     float scale_log2;
+    bool o_wide;                        /* o starts on 8 bytes */
 };
 
 /* 16-bit values as doubles without a conversion (those run at a quarter of the multiply-adds' rate): the exponent and
  * mantissa bits moved to their place in a double's high word, which is the value times 2^-896 (bf16) or 2^-1008 (fp16),
- * subnormals included.  The query sum carries 2^800 or 2^900, so a score comes out times 2^-SHIFT.  An infinity or a NaN
- * would come out finite: `special` collects the magnitudes, and a mean that has one is summed again by conversion. */
+ * subnormals included.  The query sum carries 2^800 or 2^900, so a score comes out times 2^-SHIFT.  An infinity
+ * or a NaN would come out finite: `special` collects the magnitudes, and a mean that has one is summed again by conversion. */
 template <int DT> struct Wide;
 template <> struct Wide<SV_DTYPE_BF16> {
     static constexpr int SHIFT = 96;
@@ -93,155 +96,80 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
     const unsigned long long b = (unsigned long long)__double_as_longlong(s + 0.0);       /* -0 + 0 = +0: equal scores, equal keys */
     return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
-/* A float that orders as the key does (not strictly): the score's sign, its exponent brought back by SHIFT, 23 bits; what
- * is too small is 0, what is too great (an infinity) the greatest float. */
-template <int SHIFT>
-__device__ __forceinline__ float key_float(unsigned long long key) {
-    const uint32_t k = (uint32_t)(key >> 32), b = (k >> 31) ? k & 0x7FFFFFFFu : ~k & 0x7FFFFFFFu;
-    const int32_t e = (int32_t)b - ((896 - SHIFT) << 20);
-    const uint32_t f = e < 0 ? 0u : (uint32_t)min(e, (255 << 20) - 1) << 3;
-    return __uint_as_float(f | ((k >> 31) ? 0u : 0x80000000u));
+/* The nearest float of a score (which carries 2^-SHIFT), as a word that orders as floats do; NaN with minus infinity. */
+template <int DT>
+__device__ __forceinline__ uint32_t score_word(double s) {
+    const float f = s == s ? (float)(s * __hiloint2double((Wide<DT>::SHIFT + 1023) << 20, 0)) : -INFINITY;
+    const uint32_t b = __float_as_uint(f + 0.f);
+    return (b >> 31) ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float word_float(uint32_t w) { return __uint_as_float((w >> 31) ? w & 0x7FFFFFFFu : ~w); }
+__device__ __forceinline__ uint32_t float_word(float f) { const uint32_t b = __float_as_uint(f); return (b >> 31) ? ~b : b | 0x80000000u; }
+#define SP_LOWEST 0x00800000u        /* the words of the finite floats */
+#define SP_GREATEST 0xFF7FFFFFu
 
 /* What the ring holds before the first tile: the scores of a chunk of blocks behind the best of the chunks before, and the
  * choice's own tables. */
 struct ChoiceSmem {
-    unsigned long long keys[SP_CAP];
-    unsigned long long list_key[SP_LIST];
-    int32_t place[SP_CAP];                 /* the block's number in the pool, -1: none */
-    uint32_t hist[256];
-    uint32_t list[SP_LIST], sure[SP_LIST];
+    uint32_t word[SP_CAP];                            /* a score as a float's word: tells all but the closest apart */
+    uint32_t key_hi[SP_CAP], key_lo[SP_CAP];          /* the score's 64-bit key */
+    int32_t place[SP_CAP];                            /* the block's number in the pool, -1: none */
+    uint32_t list[SP_LIST], list_word[SP_LIST];
     uint32_t ids[SILVANN_B200_PAGED_KEEP_MAX], picked[SILVANN_B200_PAGED_KEEP_MAX];
+    uint32_t hist[256];
     double qsum[256];
-    unsigned long long cut;
-    float lo[SP_WARPS], hi[SP_WARPS];
-    uint32_t warp_in[SP_WARPS], warp_tie[SP_WARPS];
-    uint32_t bin, need, in_bin, ties, n_list, n_sure;
-    uint8_t bins[SP_CAP];
+    uint32_t lo[SP_WARPS], hi[SP_WARPS], warp_in[SP_WARPS], warp_tie[SP_WARPS];
+    uint32_t bin, need;
+    __device__ __forceinline__ unsigned long long key(uint32_t i) const { return (unsigned long long)key_hi[i] << 32 | key_lo[i]; }
 };
 
 /* A histogram walked down from its top bin by one warp: the bin where the count reaches `need`, and what is still needed in it. */
 __device__ __forceinline__ void hist_walk(ChoiceSmem& S, uint32_t need, int lane) {
-    uint32_t h[8], mine = 0u;
-    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(S.hist + 248 - 8 * lane);
-    *reinterpret_cast<uint4*>(h + 4) = *reinterpret_cast<const uint4*>(S.hist + 252 - 8 * lane);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) mine += h[b];
+    uint32_t mine = 0u;
+    for (int b = 0; b < 8; ++b) mine += S.hist[255 - 8 * lane - b];
     uint32_t upto = mine;
-#pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
     const unsigned reached = __ballot_sync(0xffffffffu, upto >= need);
     if (lane == __ffs(reached) - 1) {
-        uint32_t covered = upto - mine;
-        bool found = false;
-#pragma unroll
-        for (int b = 7; b >= 0; --b)
-            if (!found) {
-                if (covered + h[b] >= need) { found = true; S.bin = 248u - 8u * (uint32_t)lane + b; S.need = need - covered; S.in_bin = h[b]; }
-                else covered += h[b];
-            }
+        uint32_t covered = upto - mine, bin = 255u - 8u * (uint32_t)lane;
+        for (int b = 0; b < 7 && covered + S.hist[bin] < need; ++b) covered += S.hist[bin--];
+        S.bin = bin; S.need = need - covered;
     }
 }
 
-/* The `take` greatest of keys[0..m) (equal keys: the lower index), their indexes ascending into S.picked; m > take > 0.
- * Called by SP_THREADS threads.
- * A histogram of 256 steps of equal width between the least and the greatest finite score: the bin that the last of the
- * chosen falls in rarely holds more than a few (a tail of scores is thin), and those few are ranked against each other.  Where
- * that is more than SP_LIST — many equal scores — its keys are counted a byte at a time instead, and the choice is written
- * in order by two passes over all keys, as it is for more than SP_LIST blocks. */
-template <int SHIFT>
-__device__ __noinline__ void choose(ChoiceSmem& S, uint32_t m, uint32_t take) {
+/* Where many scores are equal, or many blocks are chosen: the `take`-th greatest key found a byte at a time, then two passes
+ * over all keys, one that counts and one that writes, in index order. */
+__device__ __noinline__ void choose_by_bytes(ChoiceSmem& S, uint32_t m, uint32_t take) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float mn = INFINITY, mx = -INFINITY;
-    for (uint32_t i = tid; i < m; i += SP_THREADS) {
-        const float f = key_float<SHIFT>(S.keys[i]);
-        if (fabsf(f) < 3.0e38f) { mn = fminf(mn, f); mx = fmaxf(mx, f); }
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) { mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, x)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x)); }
-    if (lane == 0) { S.lo[warp] = mn; S.hi[warp] = mx; }
-    S.hist[tid] = 0u;
-    if (tid == 0) { S.n_list = 0u; S.n_sure = 0u; }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SP_WARPS; ++w) { mn = fminf(mn, S.lo[w]); mx = fmaxf(mx, S.hi[w]); }
-    if (!(mn < mx)) { mn = 0.f; mx = 0.f; }
-    const float per = mx > mn ? 255.99f / (mx - mn) : 0.f;
-    for (uint32_t i = tid; i < m; i += SP_THREADS) {
-        const uint32_t b = (uint32_t)min(max((int)((key_float<SHIFT>(S.keys[i]) - mn) * per), 0), 255);
-        S.bins[i] = (uint8_t)b;
-        atomicAdd(&S.hist[b], 1u);
-    }
-    __syncthreads();
-    if (warp == 0) hist_walk(S, take, lane);
-    __syncthreads();
-    const uint32_t bin = S.bin, need = S.need, in_bin = S.in_bin;
-    if (take <= SP_LIST && in_bin <= SP_LIST) {
-        /* what lies above the bin is sure; the bin's own are listed and ranked */
-        for (uint32_t i4 = tid; i4 < (m + 3u) / 4u; i4 += SP_THREADS) {
-            const uint32_t w = reinterpret_cast<const uint32_t*>(S.bins)[i4];
-            if (__vcmpgeu4(w, bin * 0x01010101u) == 0u) continue;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint32_t i = 4u * i4 + x, b = (w >> (8 * x)) & 255u;
-                if (i >= m || b < bin) continue;
-                if (b > bin) S.sure[atomicAdd(&S.n_sure, 1u)] = i;
-                else { const uint32_t z = atomicAdd(&S.n_list, 1u); S.list[z] = i; S.list_key[z] = S.keys[i]; }
-            }
-        }
-        __syncthreads();
-        if ((uint32_t)tid < in_bin) {
-            const unsigned long long k = S.list_key[tid];
-            const uint32_t i = S.list[tid];
-            uint32_t ahead = 0u;
-            for (uint32_t j = 0; j < in_bin; ++j) { const unsigned long long x = S.list_key[j]; ahead += x > k || (x == k && S.list[j] < i); }
-            if (ahead < need) S.sure[take - need + ahead] = i;
-        }
-        __syncthreads();
-        if ((uint32_t)tid < take) {
-            const uint32_t i = S.sure[tid];
-            uint32_t at = 0u, j = 0u;
-            for (; j + 4u <= take; j += 4u) { const uint4 x = *reinterpret_cast<const uint4*>(S.sure + j); at += (x.x < i) + (x.y < i) + (x.z < i) + (x.w < i); }
-            for (; j < take; ++j) at += S.sure[j] < i;
-            S.picked[at] = i;
-        }
-        __syncthreads();
-        return;
-    }
-    /* keys of that bin above `cut`, and the first `ties` of those that equal it, belong to the choice */
     unsigned long long known = 0ull, cut = 0ull;
-    uint32_t ties = need;
+    uint32_t ties = take;
     for (int shift = 56; shift >= 0; shift -= 8) {
         S.hist[tid] = 0u;
         __syncthreads();
         for (uint32_t i = tid; i < m; i += SP_THREADS)
-            if (S.bins[i] == bin && (S.keys[i] & known) == cut) atomicAdd(&S.hist[(uint32_t)(S.keys[i] >> shift) & 255u], 1u);
+            if ((S.key(i) & known) == cut) atomicAdd(&S.hist[(uint32_t)(S.key(i) >> shift) & 255u], 1u);
         __syncthreads();
         if (warp == 0) hist_walk(S, ties, lane);
         __syncthreads();
         cut |= (unsigned long long)S.bin << shift; ties = S.need; known |= 255ull << shift;
         __syncthreads();
     }
-    /* in index order: each warp owns a run of indexes; one pass counts, one writes */
+    /* every key above the cut and the first `ties` of those that equal it; each warp owns a run of indexes */
     const uint32_t run = ((m + SP_THREADS - 1) / SP_THREADS) * 32u, i0 = warp * run;
     uint32_t n_in = 0u, n_tie = 0u;
     for (uint32_t i = i0 + lane; i < i0 + run; i += 32) {
-        bool in = false, tie = false;
-        if (i < m) { const uint32_t b = S.bins[i]; in = b > bin || (b == bin && S.keys[i] > cut); tie = b == bin && S.keys[i] == cut; }
-        n_in += __popc(__ballot_sync(0xffffffffu, in)); n_tie += __popc(__ballot_sync(0xffffffffu, tie));
+        n_in += __popc(__ballot_sync(0xffffffffu, i < m && S.key(i) > cut)); n_tie += __popc(__ballot_sync(0xffffffffu, i < m && S.key(i) == cut));
     }
     if (lane == 0) { S.warp_in[warp] = n_in; S.warp_tie[warp] = n_tie; }
     __syncthreads();
     uint32_t at = 0u, tied = 0u;
-#pragma unroll
-    for (int w = 0; w < SP_WARPS; ++w) if (w < warp) { at += S.warp_in[w]; tied += S.warp_tie[w]; }
+    for (int w = 0; w < warp; ++w) { at += S.warp_in[w]; tied += S.warp_tie[w]; }
     at += min(tied, ties);
     const unsigned below = (1u << lane) - 1u;
     for (uint32_t i = i0 + lane; i < i0 + run; i += 32) {
-        bool in = false, tie = false;
-        if (i < m) { const uint32_t b = S.bins[i]; in = b > bin || (b == bin && S.keys[i] > cut); tie = b == bin && S.keys[i] == cut; }
+        const bool tie = i < m && S.key(i) == cut;
         const unsigned tb = __ballot_sync(0xffffffffu, tie);
-        in |= tie && tied + __popc(tb & below) < ties;
+        const bool in = (i < m && S.key(i) > cut) || (tie && tied + __popc(tb & below) < ties);
         const unsigned ib = __ballot_sync(0xffffffffu, in);
         if (in) S.picked[at + __popc(ib & below)] = i;
         at += __popc(ib); tied += __popc(tb);
@@ -249,22 +177,138 @@ __device__ __noinline__ void choose(ChoiceSmem& S, uint32_t m, uint32_t take) {
     __syncthreads();
 }
 
+/* A word that exactly `take` of the threads' words (K each; 0: none) reach, found by halving the interval between the least and the
+ * greatest finite one with the whole block counting, a barrier a step; or 0 when there is none: equal words lie across the border, or
+ * infinities do. */
+template <int K>
+__device__ __forceinline__ uint32_t border(ChoiceSmem& S, const uint32_t (&w)[K], uint32_t take) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t mn = 0xFFFFFFFFu, mx = 0u;
+#pragma unroll
+    for (int x = 0; x < K; ++x) {
+        if (w[x] >= SP_LOWEST && w[x] <= SP_GREATEST) { mn = min(mn, w[x]); mx = max(mx, w[x]); }
+    }
+    mn = __reduce_min_sync(0xffffffffu, mn); mx = __reduce_max_sync(0xffffffffu, mx);
+    if (lane == 0) { S.lo[warp] = mn; S.hi[warp] = mx; }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < SP_WARPS; ++x) { mn = min(mn, S.lo[x]); mx = max(mx, S.hi[x]); }
+    if (mn > mx) return 0u;
+    auto reach = [&](uint32_t t) { uint32_t c = 0u;
+#pragma unroll
+        for (int x = 0; x < K; ++x) c += __syncthreads_count(w[x] >= t);
+        return c; };
+    uint32_t c = reach(mn);
+    if (c <= take) return c == take ? mn : 0u;
+    float lo = word_float(mn), hi = word_float(mx);
+    for (int step = 0; step < 64; ++step) {
+        const float mid = 0.5f * lo + 0.5f * hi;
+        if (!(mid > lo && mid < hi)) return 0u;
+        c = reach(float_word(mid));
+        if (c == take) return float_word(mid);
+        if (c > take) lo = mid; else hi = mid;
+    }
+    return 0u;
+}
+
+/* The `take` greatest of the m keys (equal ones: the lower index), their indexes ascending into S.picked; m > take > 0.
+ * Called by SP_THREADS threads.
+ * Up to 512 keys: the border between the chosen and the others is looked for among their words.  More: first among the threads' own
+ * greatest words — `take` of them reach it, so at least `take` keys do, and, scores being in no order, not many more: they are
+ * listed, in order, and the border looked for among them.  Where there is no border (equal words on both sides of it) or the list is
+ * too long, and for more than 256 blocks, the 64-bit keys are counted a byte at a time. */
+__device__ __forceinline__ void choose(ChoiceSmem& S, uint32_t m, uint32_t take) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    uint32_t n = m;
+    const uint32_t* words = S.word;
+    if (m > SP_LIST) {
+        if (take > SP_THREADS) { choose_by_bytes(S, m, take); return; }
+        /* a thread's keys are neighbours, so that the list is in order */
+        constexpr int MOST = (SP_CAP + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u);        /* loads of four */
+        const uint32_t run = (m + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u) * 4u, i0 = tid * run;
+        uint32_t best[1] = {0u};
+#pragma unroll
+        for (int x = 0; x < MOST; ++x)
+            if (4u * x < run && i0 + 4u * x < m) { const uint4 y = *reinterpret_cast<const uint4*>(S.word + i0 + 4 * x); best[0] = max(best[0], max(max(y.x, y.y), max(y.z, y.w))); }
+        const uint32_t least = border<1>(S, best, take);
+        uint32_t hits = 0u;
+#pragma unroll
+        for (int x = 0; x < MOST; ++x)
+            if (4u * x < run && i0 + 4u * x < m) {
+                const uint4 y = *reinterpret_cast<const uint4*>(S.word + i0 + 4 * x);
+                hits |= ((y.x >= least ? 1u : 0u) | (y.y >= least ? 2u : 0u) | (y.z >= least ? 4u : 0u) | (y.w >= least ? 8u : 0u)) << (4 * x);
+            }
+        uint32_t upto = __popc(hits);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
+        if (lane == 31u) S.warp_in[warp] = upto;
+        __syncthreads();
+        uint32_t at = upto - __popc(hits);
+        n = 0u;
+#pragma unroll
+        for (uint32_t w = 0; w < SP_WARPS; ++w) { const uint32_t c = S.warp_in[w]; if (w < warp) at += c; n += c; }
+        if (least == 0u || n > SP_LIST) { __syncthreads(); choose_by_bytes(S, m, take); return; }
+        for (; hits; hits &= hits - 1u, ++at) { const uint32_t i = i0 + __ffs(hits) - 1u; S.list[at] = i; S.list_word[at] = S.word[i]; }
+        __syncthreads();
+        words = S.list_word;
+    }
+    uint32_t least;
+    uint32_t w[2] = {2u * tid < n ? words[2u * tid] : 0u, 2u * tid + 1u < n ? words[2u * tid + 1u] : 0u};
+    if (n <= SP_THREADS) {
+        uint32_t one[1] = {tid < n ? words[tid] : 0u};
+        least = border<1>(S, one, take);
+        w[0] = one[0]; w[1] = 0u;
+    } else least = border<2>(S, w, take);
+    if (least == 0u) { __syncthreads(); choose_by_bytes(S, m, take); return; }
+    const bool in0 = w[0] >= least, in1 = w[1] >= least;
+    const unsigned b0 = __ballot_sync(0xffffffffu, in0), b1 = __ballot_sync(0xffffffffu, in1), below = (1u << lane) - 1u;
+    if (lane == 0u) S.warp_in[warp] = __popc(b0) + __popc(b1);
+    __syncthreads();
+    uint32_t at = __popc(b0 & below) + __popc(b1 & below);
+#pragma unroll
+    for (uint32_t x = 0; x < SP_WARPS; ++x) if (x < warp) at += S.warp_in[x];
+    const uint32_t k = n <= SP_THREADS ? tid : 2u * tid;
+    if (in0) S.picked[at++] = words == S.word ? k : S.list[k];
+    if (in1) S.picked[at] = words == S.word ? k + 1u : S.list[k + 1u];
+    __syncthreads();
+}
+
+/* The score of a mean that holds an infinity or a NaN (any of a warp's `count`): summed by conversion.  Such a score is no finite number
+ * whatever the order, so the order is the warp's own.  Answers the score of mean `want`, or `v` where that is an ordinary one. */
+template <int D, int DT>
+__device__ __noinline__ double special_score(const uint16_t* means, uint32_t row_elems, int32_t mine, int count, const double* qsum, int want, double v, int lpb) {
+    using E = Elem<DT>;
+    const int lane = threadIdx.x & 31;
+    for (int b = 0; b < count; ++b) {
+        const int32_t at = __shfl_sync(0xffffffffu, mine, b);
+        if (at < 0) continue;
+        bool is = false;
+        double a = 0;
+        for (int e = lane; e < D; e += 32) {
+            const uint16_t h = means[(size_t)at * row_elems + e];
+            is |= (h & 0x7FFFu) >= Wide<DT>::SPECIAL;
+            const int ch = e / 8;
+            a += (double)E::to_float(h) * qsum[(((ch / lpb) * 4 + (e % 8) / 2) * lpb + ch % lpb) * 2 + e % 2];
+        }
+        for (int x = 16; x > 0; x >>= 1) a += __shfl_xor_sync(0xffffffffu, a, x);
+        if (__any_sync(0xffffffffu, is) && b == want) v = a;
+    }
+    return v;
+}
+
 __device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
     return remote;
 }
-__device__ __forceinline__ void st_cluster_u64(uint32_t at, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
-__device__ __forceinline__ void st_cluster_u32(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
-__device__ __forceinline__ void st_cluster_f32(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
 
 template <int D, int DT, int NHT>
-__global__ void __launch_bounds__(SP_THREADS, D == 256 ? 1 : 2)
+__global__ void __launch_bounds__(SP_THREADS, 2)
 paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const SparseParams P) {
     using Cfg = SparseCfg<D>;
     using E = Elem<DT>;
     using W = Wide<DT>;
-    constexpr int HPB = 8 * NHT, KS = D / 16, NW = SP_WARPS, VS = KS / 2;      /* VS: 16-column steps of the value product a warp */
+    constexpr int HPB = 8 * NHT, KS = D / 16, NW = SP_WARPS, PW = Cfg::PW, VS = KS / (NW / PW);      /* VS: 16-column steps of the value product a warp */
     constexpr int Q_BYTES = Cfg::BOXES * HPB * 128;
     constexpr bool QREG = NHT == 1;          /* 16 heads: the query's fragments are read from shared memory again for every tile */
 
@@ -332,9 +376,12 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     /* a peer's shared memory may be written only once the peer runs: arrive now, wait ahead of the first score */
     if (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
-    /* Means are dealt to the cluster's warps BPS at a time, U times round: mean `i` of this lane's u-th is
-     * i0 + u * STRIDE + (its warp's place) * BPS + lane / LPB.  Lane l looks up the page of the (l / BPS)-th round's l % BPS-th. */
-    const uint32_t STRIDE = CL * NW * Cfg::BPS, w_at = (crank * NW + warp) * Cfg::BPS;
+    /* A chunk's means are cut evenly over the cluster (in fours: its scores are sent round sixteen bytes at a time); a thread block's
+     * `n` from `base` on are dealt to its warps BPS at a time, U times round: this lane's u-th is i0 + u * STRIDE + w_at + lane / LPB.
+     * Lane l looks up the page of the (l / BPS)-th round's l % BPS-th. */
+    constexpr uint32_t STRIDE = NW * Cfg::BPS;
+    const uint32_t w_at = warp * Cfg::BPS;
+    auto share = [&](uint32_t chunk) { return ((chunk + CL - 1u) / CL + 3u) & ~3u; };
     auto look_up = [&](uint32_t base, uint32_t n, uint32_t i0) {
         const uint32_t i = i0 + (lane / Cfg::BPS) * STRIDE + w_at + lane % Cfg::BPS;
         if (lane >= Cfg::WB || i >= n) return -1;
@@ -353,8 +400,13 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         }
     };
     int32_t mine = -1, next = -1;
+    /* the blocks that are always attended: their pages are asked for first, and kept below while the means are on their way */
+    auto always = [&](uint32_t i) { return i < c.lo ? i : c.hi + (i - c.lo - c.take); };
+    const bool fixed = (uint32_t)tid < c.count && !((uint32_t)tid >= c.lo && (uint32_t)tid < c.lo + c.take);
+    const int32_t fixed_at = fixed ? paged_block(row, P.stride, P.pool_pages, P.per, always(tid)) : 0;
     if (c.take) {
-        mine = look_up(c.lo, min(SP_CHUNK, c.hi - c.lo), 0u);
+        const uint32_t chunk = min(SP_CHUNK, c.hi - c.lo), per = share(chunk), from = min(chunk, crank * per);
+        mine = look_up(c.lo + from, min(per, chunk - from), 0u);
         load(mine);
     }
 #pragma unroll
@@ -364,17 +416,14 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     }
     /* the summed query in pairs, a round's pairs side by side for the lanes that share a mean */
     if (P.top && tid < D) S.qsum[((((tid / 8) / Cfg::LPB) * 4 + (tid % 8) / 2) * Cfg::LPB + (tid / 8) % Cfg::LPB) * 2 + tid % 2] = qs * W::up();
-    /* the blocks that are always attended, while the means are on their way */
     for (uint32_t i = tid; i < keep; i += SP_THREADS) {
         if (i >= c.lo && i < c.lo + c.take) continue;
-        int32_t id = -1;
         if (i < c.count) {
-            id = i < c.lo ? (int32_t)i : (int32_t)(c.hi + (i - c.lo - c.take));
-            const int32_t at = paged_block(row, P.stride, P.pool_pages, P.per, (uint32_t)id);
+            const int32_t at = i == (uint32_t)tid ? fixed_at : paged_block(row, P.stride, P.pool_pages, P.per, always(i));
             bad |= at < 0;
             slots[i] = slot_of(at);
         }
-        if (chosen) chosen[i] = id;
+        if (chosen) chosen[i] = i < c.count ? (int32_t)always(i) : -1;
     }
     __syncthreads();
     if (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -382,46 +431,33 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     /* ---- scores and choice, a chunk of blocks at a time ---- */
     uint32_t have = 0;                                                    /* the best of the chunks so far: keys, place, ids [0..have) */
     for (uint32_t base = c.lo; c.take && base < c.hi; base += SP_CHUNK) {
-        const uint32_t n = min(SP_CHUNK, c.hi - base);
+        const uint32_t chunk = min(SP_CHUNK, c.hi - base), per = share(chunk), from = min(chunk, crank * per), n = min(per, chunk - from);
+        const uint32_t front = (have + 3u) & ~3u;                         /* where the chunk's scores begin, on sixteen bytes */
         {
-            if (base != c.lo) { mine = look_up(base, n, 0u); load(mine); }
+            if (base != c.lo) { mine = look_up(base + from, n, 0u); load(mine); }
             for (uint32_t i0 = 0; i0 < n; i0 += STRIDE * Cfg::U) {
-                next = look_up(base, n, i0 + STRIDE * Cfg::U);
+                next = look_up(base + from, n, i0 + STRIDE * Cfg::U);
                 double s[Cfg::U];
+                uint32_t special = 0u;
 #pragma unroll
                 for (int g = 0; g < Cfg::U; g += 4) {
                     s[g] = s[g + 1] = s[g + 2] = s[g + 3] = 0;
                     if (i0 + g * STRIDE + w_at >= n) continue;
-                    uint32_t special = 0u;
 #pragma unroll
-                    for (int y = 0; y < Cfg::CPL; ++y)
+                    for (int y = 0; y < Cfg::CPL; ++y) {
+                        double a[4] = {0, 0, 0, 0};
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
                             const double2 q2 = *reinterpret_cast<const double2*>(S.qsum + ((y * 4 + z) * Cfg::LPB + lane % Cfg::LPB) * 2);
 #pragma unroll
                             for (int u = g; u < g + 4; ++u) {
                                 const uint32_t w = z == 0 ? x[u][y].x : z == 1 ? x[u][y].y : z == 2 ? x[u][y].z : x[u][y].w;
-                                s[u] = fma(W::lo(w), q2.x, s[u]); s[u] = fma(W::hi(w), q2.y, s[u]);
+                                a[u - g] = fma(W::lo(w), q2.x, a[u - g]); a[u - g] = fma(W::hi(w), q2.y, a[u - g]);
                                 special = __vmaxu2(special, w & 0x7FFF7FFFu);
                             }
                         }
-                    if ((special & 0xFFFFu) >= W::SPECIAL || (special >> 16) >= W::SPECIAL) {
 #pragma unroll
-                        for (int u = g; u < g + 4; ++u) {
-                            double a = 0;
-                            bool is = false;
-#pragma unroll
-                            for (int y = 0; y < Cfg::CPL; ++y)
-#pragma unroll
-                                for (int z = 0; z < 4; ++z) {
-                                    const uint32_t w = z == 0 ? x[u][y].x : z == 1 ? x[u][y].y : z == 2 ? x[u][y].z : x[u][y].w;
-                                    const float2 f = E::unpack2(w);
-                                    const double2 q2 = *reinterpret_cast<const double2*>(S.qsum + ((y * 4 + z) * Cfg::LPB + lane % Cfg::LPB) * 2);
-                                    a += (double)f.x * q2.x; a += (double)f.y * q2.y;
-                                    is |= (w & 0x7FFFu) >= W::SPECIAL || ((w >> 16) & 0x7FFFu) >= W::SPECIAL;
-                                }
-                            if (is) s[u] = a;
-                        }
+                        for (int u = 0; u < 4; ++u) s[g + u] += a[u];
                     }
                 }
                 const int32_t old = mine;
@@ -440,58 +476,73 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 if (T2 == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
                 const int u = (up0 ? 4 : 0) + (up1 ? 2 : 0) + (up2 ? 1 : 0);
                 const int32_t at = __shfl_sync(0xffffffffu, old, u * Cfg::BPS + lane / Cfg::LPB);
+                if (__any_sync(0xffffffffu, (special & 0xFFFFu) >= W::SPECIAL || (special >> 16) >= W::SPECIAL))
+                    v = special_score<D, DT>(P.means + (size_t)kvh * D, P.kv_heads * D, old, Cfg::WB, S.qsum, u * Cfg::BPS + lane / Cfg::LPB, v, Cfg::LPB);
                 const uint32_t i = i0 + u * STRIDE + w_at + lane / Cfg::LPB;
-                if (i < n) {
-                    const unsigned long long k = score_key(at >= 0 ? v : -INFINITY);
-                    if (CL == 1) { if (lane % T2 == 0) { S.keys[have + i] = k; S.place[have + i] = at; } }
-                    else for (uint32_t to = lane % T2; to < CL; to += T2) { st_cluster_u64(peer_addr(&S.keys[have + i], to), k); st_cluster_u32(peer_addr(&S.place[have + i], to), (uint32_t)at); }
+                if (i < n && lane % T2 == 0) {
+                    const double score = at >= 0 ? v : -INFINITY;
+                    const unsigned long long k = score_key(score);
+                    const uint32_t z = front + from + i;
+                    S.word[z] = score_word<DT>(score); S.key_hi[z] = (uint32_t)(k >> 32); S.key_lo[z] = (uint32_t)k; S.place[z] = at;
                 }
             }
         }
-        if (CL > 1) cluster_sync_all(); else __syncthreads();
-        const uint32_t m = have + n;
+        /* between the best of the chunks before and this chunk, and behind it: words and keys that no score has */
+        if (tid < 4u) {
+            if (have + tid < front) { S.word[have + tid] = 0u; S.key_hi[have + tid] = 0u; S.key_lo[have + tid] = 0u; }
+            S.word[front + chunk + tid] = 0u; S.key_hi[front + chunk + tid] = 0u; S.key_lo[front + chunk + tid] = 0u;
+        }
+        if (CL > 1) {
+            __syncthreads();
+            /* this block's scores to every peer (what lies behind the chunk's last is zeros there as well) */
+            const uint32_t quads = (n + 3u) / 4u;
+            for (uint32_t z = tid; z < quads * 4u * CL; z += SP_THREADS) {
+                const uint32_t to = z / (quads * 4u), a = z / quads % 4u, at = front + from + z % quads * 4u;
+                const uint32_t* src = a == 0u ? S.word : a == 1u ? S.key_hi : a == 2u ? S.key_lo : (const uint32_t*)S.place;
+                if (to == crank) continue;
+                const uint4 y = *reinterpret_cast<const uint4*>(src + at);
+                asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(peer_addr(src + at, to)), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+            }
+            cluster_sync_all();
+        } else __syncthreads();
+        const uint32_t m = front + chunk;
         const bool more = base + SP_CHUNK < c.hi;
-        {
-            if (m <= c.take) {
-                for (uint32_t i = tid; i < n; i += SP_THREADS) S.ids[have + i] = base + i;
-            } else {
-                choose<W::SHIFT>(S, m, c.take);
-                auto id_of = [&](uint32_t i) { return i < have ? S.ids[i] : base + (i - have); };
-                if (more) {
-                    /* the chosen move to the front, in order: read all, then write */
-                    constexpr int KP = SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS;
-                    unsigned long long kk[KP];
-                    uint32_t ii[KP];
-                    int32_t pp[KP];
+        /* (a chunk holds more blocks than can be chosen, or all there are: m > take) */
+        choose(S, m, c.take);
+        auto id_of = [&](uint32_t i) { return i < have ? S.ids[i] : base + (i - front); };
+        if (more) {
+            /* the chosen move to the front, in order: read all, then write */
+            constexpr int KP = SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS;
+            uint32_t kw[KP], kh[KP], kl[KP], ii[KP];
+            int32_t pp[KP];
 #pragma unroll
-                    for (int z = 0; z < KP; ++z) {
-                        const uint32_t i = tid + z * SP_THREADS;
-                        if (i < c.take) { const uint32_t at = S.picked[i]; kk[z] = S.keys[at]; ii[z] = id_of(at); pp[z] = S.place[at]; }
-                    }
-                    __syncthreads();
+            for (int z = 0; z < KP; ++z) {
+                const uint32_t i = tid + z * SP_THREADS;
+                if (i < c.take) { const uint32_t at = S.picked[i]; kw[z] = S.word[at]; kh[z] = S.key_hi[at]; kl[z] = S.key_lo[at]; ii[z] = id_of(at); pp[z] = S.place[at]; }
+            }
+            __syncthreads();
 #pragma unroll
-                    for (int z = 0; z < KP; ++z) {
-                        const uint32_t i = tid + z * SP_THREADS;
-                        if (i < c.take) { S.keys[i] = kk[z]; S.ids[i] = ii[z]; S.place[i] = pp[z]; }
-                    }
-                } else {
-                    for (uint32_t i = tid; i < c.take; i += SP_THREADS) {
-                        const uint32_t at = S.picked[i];
-                        slots[c.lo + i] = slot_of(S.place[at]);
-                        if (chosen) chosen[c.lo + i] = (int32_t)id_of(at);
-                    }
-                }
+            for (int z = 0; z < KP; ++z) {
+                const uint32_t i = tid + z * SP_THREADS;
+                if (i < c.take) { S.word[i] = kw[z]; S.key_hi[i] = kh[z]; S.key_lo[i] = kl[z]; S.ids[i] = ii[z]; S.place[i] = pp[z]; }
+            }
+            have = c.take;
+            /* no one writes the next scores over what a peer still reads */
+            if (CL > 1) cluster_sync_all(); else __syncthreads();
+        } else {
+            for (uint32_t i = tid; i < c.take; i += SP_THREADS) {
+                const uint32_t at = S.picked[i];
+                slots[c.lo + i] = slot_of(S.place[at]);
+                if (chosen) chosen[c.lo + i] = (int32_t)id_of(at);
             }
         }
-        have = min(m, c.take);
-        if (more) { if (CL > 1) cluster_sync_all(); else __syncthreads(); }       /* no one writes the next scores over what a peer still reads */
     }
     fence_proxy_async_smem();            /* the scores' accesses to the ring come before the loads into it */
     __syncthreads();
 
     /* ---- attend: tile t of the chosen positions belongs to thread block t % CL ---- */
     const uint32_t live = (c.count - 1u) * P.block + (uint32_t)pos % P.block + 1u;      /* the row's own block is the last and may end early */
-    const uint32_t tiles = (live + 63u) / 64u;
+    const uint32_t tiles = (live + Cfg::TP - 1u) / Cfg::TP;
     const int nt = tiles > crank ? (int)((tiles - crank + CL - 1) / CL) : 0;
 
     float m_run[NHT][2], l_run[NHT][2], oacc[NHT][VS][4];
@@ -501,12 +552,12 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
         for (int k = 0; k < VS; ++k) { oacc[n][k][0] = oacc[n][k][1] = oacc[n][k][2] = oacc[n][k][3] = 0.f; }
     }
-    /* the loads of tile `it`: one box of 64 columns by min(B, 64) positions a lane of one warp */
-    const uint32_t br = min(P.block, 64u), sub = 64u / br;
+    /* the loads of tile `it`: one box of 64 columns by min(B, TP) positions a lane of one warp */
+    const uint32_t br = min(P.block, (uint32_t)Cfg::TP), sub = Cfg::TP / br;
     const uint64_t pol = l2_policy_evict_first();
     auto fetch = [&](int it) {
         const int s = it % Cfg::STAGES;
-        const uint32_t p0 = (crank + it * CL) * 64u;
+        const uint32_t p0 = (crank + it * CL) * Cfg::TP;
         const uint32_t boxes = min(sub, (live - p0 + br - 1u) / br);
         uint8_t* st = ring + s * Cfg::STAGE_BYTES;
         if (lane == 0) mbar_expect_tx(&full[s], boxes * br * 128u * Cfg::BOXES * 2u);
@@ -534,7 +585,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) load_qfrag(0, kk, qf[kk][0], qf[kk][1]);
         }
-        const int r_lo = lane >> 2, w4 = warp & 3, half = warp >> 2;      /* positions [16 w4, +16) of a tile, value columns [half D/2, +D/2) */
+        const int r_lo = lane >> 2, wp = warp % PW, wc = warp / PW;      /* positions [16 wp, +16) of a tile, value columns [16 VS wc, +16 VS) */
         for (int it = 0; it < nt; ++it) {
             const int s = it % Cfg::STAGES;
             /* the warps take turns to ask for the tile that goes where the one before this lay, once all have left it */
@@ -545,13 +596,13 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             if (!mbar_wait(&full[s], (it / Cfg::STAGES) & 1, abort_flag, P.status)) break;
             uint8_t* stage = ring + s * Cfg::STAGE_BYTES;
             const uint32_t kst = smem_u32(stage), vst = kst + Cfg::K_BYTES;
-            const uint32_t p0 = (crank + it * CL) * 64u + w4 * 16u;
+            const uint32_t p0 = (crank + it * CL) * Cfg::TP + wp * 16u;
             /* rows of V behind the row's own position may hold anything: zero, so that a zero weight times a NaN cannot reach the sum */
             if (p0 + 16u > live) {
-                for (int i = lane; i < 16 * (D / 16); i += 32) {
-                    const int y = i / (D / 16), j = half * (D / 16) + i % (D / 16);
+                for (int i = lane; i < 16 * (VS * 2); i += 32) {
+                    const int y = i / (VS * 2), j = wc * (VS * 2) + i % (VS * 2);
                     if (p0 + y >= live)
-                        *reinterpret_cast<uint4*>(stage + Cfg::K_BYTES + (j / 8) * Cfg::BOX_BYTES + swz128(w4 * 16 + y, j % 8)) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(stage + Cfg::K_BYTES + (j / 8) * Cfg::BOX_BYTES + swz128(wp * 16 + y, j % 8)) = make_uint4(0u, 0u, 0u, 0u);
                 }
                 __syncwarp();
             }
@@ -561,7 +612,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             for (int n = 0; n < NHT; ++n) { sa[n][0] = sa[n][1] = sa[n][2] = sa[n][3] = 0.f; sb[n][0] = sb[n][1] = sb[n][2] = sb[n][3] = 0.f; }
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
-                const int krow = w4 * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, chunk = 2 * kk + (lane >> 4);
+                const int krow = wp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, chunk = 2 * kk + (lane >> 4);
                 uint32_t a0, a1, a2, a3;
                 ldsm_x4(kst + (chunk / 8) * Cfg::BOX_BYTES + swz128(krow, chunk % 8), a0, a1, a2, a3);
 #pragma unroll
@@ -608,7 +659,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             /* O^T[value column][head] += V_tile^T P^T */
 #pragma unroll
             for (int mt = 0; mt < VS; ++mt) {
-                const int j = lane >> 3, vrow = w4 * 16 + (lane & 7) + (j >> 1) * 8, chunk = 2 * (half * VS + mt) + (j & 1);
+                const int j = lane >> 3, vrow = wp * 16 + (lane & 7) + (j >> 1) * 8, chunk = 2 * (wc * VS + mt) + (j & 1);
                 uint32_t a0, a1, a2, a3;
                 ldsm_x4_t(vst + (chunk / 8) * Cfg::BOX_BYTES + swz128(vrow, chunk % 8), a0, a1, a2, a3);
 #pragma unroll
@@ -642,68 +693,96 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
         __syncthreads();
     }
-    constexpr int PW = NW / 2;                        /* warps that split a tile by positions */
+    constexpr int WS = D + 4;                         /* a row of partials: the pad spreads the accumulators' columns over the banks */
     float* wm = (float*)ring;                         /* [PW][HPB] */
     float* wl = wm + PW * HPB;                        /* [PW][HPB] */
-    float* wo = wl + PW * HPB;                        /* [PW][HPB][D] */
+    float* wo = wl + PW * HPB;                        /* [PW][HPB][WS] */
     {
-        const int r_lo = lane >> 2, c2 = (lane & 3) * 2, w4 = warp & 3, half = warp >> 2;
+        const int r_lo = lane >> 2, c2 = (lane & 3) * 2, wp = warp % PW, wc = warp / PW;
 #pragma unroll
         for (int n = 0; n < NHT; ++n) {
             const int ha = n * 8 + c2;
-            if (r_lo == 0 && half == 0) {
-                wm[w4 * HPB + ha] = m_run[n][0]; wm[w4 * HPB + ha + 1] = m_run[n][1];
-                wl[w4 * HPB + ha] = l_run[n][0]; wl[w4 * HPB + ha + 1] = l_run[n][1];
+            if (r_lo == 0 && wc == 0) {
+                wm[wp * HPB + ha] = m_run[n][0]; wm[wp * HPB + ha + 1] = m_run[n][1];
+                wl[wp * HPB + ha] = l_run[n][0]; wl[wp * HPB + ha + 1] = l_run[n][1];
             }
 #pragma unroll
             for (int k = 0; k < VS; ++k) {
-                float* at = wo + (size_t)(w4 * HPB) * D + (half * VS + k) * 16 + r_lo;
-                at[(ha) * D] = oacc[n][k][0];
-                at[(ha + 1) * D] = oacc[n][k][1];
-                at[(ha) * D + 8] = oacc[n][k][2];
-                at[(ha + 1) * D + 8] = oacc[n][k][3];
+                float* at = wo + (wp * HPB + ha) * WS + (wc * VS + k) * 16 + r_lo;
+                at[0] = oacc[n][k][0];
+                at[WS] = oacc[n][k][1];
+                at[8] = oacc[n][k][2];
+                at[WS + 8] = oacc[n][k][3];
             }
         }
     }
     __syncthreads();
     bool hit = false;
-    auto answer = [&](uint32_t h, uint32_t e, float m, float l, float acc) {
+    /* four columns of a head's answer */
+    auto answer = [&](uint32_t h, uint32_t e, float m, float l, const float (&acc)[4]) {
         const size_t hq = out0 + h;
-        if (P.o) ((uint16_t*)P.o)[hq * D + e] = E::from_float(acc / l, hit);
-        if (P.res) { float* x = P.res + hq * (D + 2); x[2 + e] = acc; if (e == 0) { x[0] = m * SV_LN2; x[1] = l; } }
-    };
-    for (uint32_t i = tid; i < heads * D; i += blockDim.x) {
-        const uint32_t h = i / D, e = i % D;
-        float m = -INFINITY;
+        if (P.o) {
+            const float inv = 1.0f / l;
+            uint16_t w[4];
 #pragma unroll
-        for (int w = 0; w < PW; ++w) m = fmaxf(m, wm[w * HPB + h]);
-        float acc = 0.f, l = 0.f;
+            for (int x = 0; x < 4; ++x) w[x] = E::from_float(acc[x] * inv, hit);
+            uint16_t* at = (uint16_t*)P.o + hq * D + e;
+            if (P.o_wide) *reinterpret_cast<uint2*>(at) = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
+            else { at[0] = w[0]; at[1] = w[1]; at[2] = w[2]; at[3] = w[3]; }
+        }
+        if (P.res) {
+            float* at = P.res + hq * (D + 2);
+            at[2 + e] = acc[0]; at[3 + e] = acc[1]; at[4 + e] = acc[2]; at[5 + e] = acc[3];
+            if (e == 0) { at[0] = m * SV_LN2; at[1] = l; }
+        }
+    };
+    for (uint32_t i = tid; i < heads * (D / 4); i += SP_THREADS) {
+        const uint32_t h = i / (D / 4), e = i % (D / 4) * 4u;
+        float pm[PW], m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PW; ++w) { pm[w] = wm[w * HPB + h]; m = fmaxf(m, pm[w]); }
+        float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
 #pragma unroll
         for (int w = 0; w < PW; ++w) {
-            const float mw = wm[w * HPB + h];
-            if (mw != -INFINITY) { const float f = fast_exp2(mw - m); acc += wo[(size_t)(w * HPB + h) * D + e] * f; l += wl[w * HPB + h] * f; }
+            const float f = pm[w] == -INFINITY ? 0.f : fast_exp2(pm[w] - m);
+            const float4 x = *reinterpret_cast<const float4*>(wo + (w * HPB + h) * WS + e);
+            acc[0] += x.x * f; acc[1] += x.y * f; acc[2] += x.z * f; acc[3] += x.w * f; l += wl[w * HPB + h] * f;
         }
         if (CL == 1) answer(h, e, m, l, acc);
         else {
             /* columns [c D/CL, (c+1) D/CL) of every head meet in thread block c */
             const uint32_t DS = D / CL, to = e / DS;
-            st_cluster_f32(peer_addr(meet + (crank * HPB + h) * DS + e % DS, to), acc);
-            if (e % DS == 0) { st_cluster_f32(peer_addr(meet_ml + (crank * HPB + h) * 2, to), m); st_cluster_f32(peer_addr(meet_ml + (crank * HPB + h) * 2 + 1, to), l); }
+            const uint32_t at = peer_addr(meet + (crank * HPB + h) * DS + e % DS, to);
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(acc[0]), "f"(acc[1]), "f"(acc[2]), "f"(acc[3]) : "memory");
+            if (e % DS == 0) asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(peer_addr(meet_ml + (crank * HPB + h) * 2, to)), "f"(m), "f"(l) : "memory");
         }
     }
     if (CL > 1) {
         cluster_sync_all();                           /* nothing is sent to a peer after this */
         const uint32_t DS = D / CL;
-        for (uint32_t i = tid; i < heads * DS; i += blockDim.x) {
-            const uint32_t h = i / DS, e = i % DS;
-            float m = -INFINITY;
-            for (uint32_t x = 0; x < CL; ++x) m = fmaxf(m, meet_ml[(x * HPB + h) * 2]);
-            float acc = 0.f, l = 0.f;
-            for (uint32_t x = 0; x < CL; ++x) {
-                const float mx = meet_ml[(x * HPB + h) * 2], f = mx == -INFINITY ? 0.f : fast_exp2(mx - m);
-                acc += meet[(x * HPB + h) * DS + e] * f; l += meet_ml[(x * HPB + h) * 2 + 1] * f;
+        /* four lanes share four columns of a head: each folds every fourth peer, then they fold each other's */
+        for (uint32_t i0 = 0; i0 < heads * DS; i0 += SP_THREADS) {
+            const uint32_t i = min(i0 + tid, heads * DS - 1u), part = i & 3u, h = i / DS, e = i % DS & ~3u;
+            float2 ml[4];
+            float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t x = 0; x < 4u; ++x) { ml[x] = part + 4u * x < CL ? *reinterpret_cast<const float2*>(meet_ml + ((part + 4u * x) * HPB + h) * 2) : make_float2(-INFINITY, 0.f); m = fmaxf(m, ml[x].x); }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+#pragma unroll
+            for (uint32_t x = 0; x < 4u; ++x)
+                if (part + 4u * x < CL) {
+                    const float f = ml[x].x == -INFINITY ? 0.f : fast_exp2(ml[x].x - m);
+                    const float4 y = *reinterpret_cast<const float4*>(meet + ((part + 4u * x) * HPB + h) * DS + e);
+                    acc[0] += y.x * f; acc[1] += y.y * f; acc[2] += y.z * f; acc[3] += y.w * f; l += ml[x].y * f;
+                }
+#pragma unroll
+            for (int t = 1; t < 4; t <<= 1) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) acc[y] += __shfl_xor_sync(0xffffffffu, acc[y], t);
+                l += __shfl_xor_sync(0xffffffffu, l, t);
             }
-            answer(h, crank * DS + e, m, l, acc);
+            if (part == 0 && i0 + tid < heads * DS) answer(h, crank * DS + e, m, l, acc);
         }
     }
     if (hit && P.over) atomicOr(P.over, SV_FAULT_OVERFLOW);
@@ -718,7 +797,7 @@ static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& v
     const size_t smem = fixed + (size_t)keep * 4;
     static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= sizeof(ChoiceSmem), "the scores fit the ring");
     static_assert(fixed + SILVANN_B200_PAGED_KEEP_MAX * 4 <= 227 * 1024, "a thread block's shared memory");
-    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (size_t)(SP_WARPS / 2) * 8 * NHT * (D + 2) * 4, "the partials fit the ring");
+    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (size_t)Cfg::PW * 8 * NHT * (D + 6) * 4, "the partials fit the ring");
     static std::atomic<bool> attr_set[SPARSE_DEVICES];
     int d = 0; cudaGetDevice(&d);
     if (d >= 0 && d < SPARSE_DEVICES && !attr_set[d].load(std::memory_order_acquire)) {
@@ -747,13 +826,13 @@ static cudaError_t sparse_launch(SparseParams& P, const void* k, const void* v, 
     const uint32_t nht = P.group <= 8u ? 1u : 2u;
     P.head_blocks = (P.group + 8u * nht - 1u) / (8u * nht);
     const uint64_t units = (uint64_t)rows * P.kv_heads * P.head_blocks, cols = (uint64_t)P.kv_heads * d;
-    /* As many thread blocks a row as keep every SM busy once (twice where two fit one), as far as a row's longest list of tiles goes round. */
-    const uint32_t sms = device_sm_count() * (d == 256 ? 1u : 2u), tiles = ((P.first + P.last + P.top) * P.block + 63u) / 64u;
+    /* As many thread blocks a row as fit the card at once, two an SM, as far as a row's longest list of tiles goes round. */
+    const uint32_t sms = device_sm_count() * 2u, tp = d == 256 ? 32u : 64u, tiles = ((P.first + P.last + P.top) * P.block + tp - 1u) / tp;
     uint32_t cluster = 1u;
     while (cluster < 16u && units * cluster * 2u <= sms && cluster < tiles) cluster *= 2u;
     CUtensorMap km, vm;
     const bool bf = dtype == SV_DTYPE_BF16;
-    const uint32_t box = P.block < 64u ? P.block : 64u;
+    const uint32_t box = P.block < tp ? P.block : tp;
     if (!make_map_2d_sw128(&km, k, cols, (uint64_t)P.pool_pages * P.page_pos, cols * 2u, 64u, box, bf) || !make_map_2d_sw128(&vm, v, cols, (uint64_t)P.pool_pages * P.page_pos, cols * 2u, 64u, box, bf))
         return cudaErrorInvalidValue;
 #define SV_SPARSE_CASE(DD, TT) return nht == 1u ? sparse_launch_one<DD, TT, 1>(km, vm, P, units, cluster, st) : sparse_launch_one<DD, TT, 2>(km, vm, P, units, cluster, st)
@@ -794,7 +873,7 @@ SV_EXPORT int silvann_b200_paged_sparse(void* o, float* res, int32_t* chosen, co
     P.o = o; P.res = res; P.chosen = chosen; P.q = (const uint16_t*)q; P.means = (const uint16_t*)k_means;
     P.row_seq = row_seq; P.row_pos = row_pos; P.table = page_table; P.over = over; P.status = sv::device_status_word(); P.q_stride = q_stride; P.seqs = seqs;
     P.stride = table_stride; P.pool_pages = (uint32_t)pool_pages; P.page_pos = page_positions; P.block = block_positions; P.per = sv::paged_div(page_positions / block_positions); P.q_heads = q_heads; P.kv_heads = kv_heads;
-    P.group = q_heads / kv_heads; P.first = first; P.last = last; P.top = top; P.scale_log2 = (1.0f / sqrtf((float)head_dim)) * SV_LOG2E;
+    P.group = q_heads / kv_heads; P.first = first; P.last = last; P.top = top; P.o_wide = aligned(o, 8); P.scale_log2 = (1.0f / sqrtf((float)head_dim)) * SV_LOG2E;
     cudaError_t e = sv::sparse_launch(P, k_pool, v_pool, rows, head_dim, dtype, (cudaStream_t)stream);
     if (e == cudaSuccess) return SILVANN_B200_OK;
     (void)cudaGetLastError();

@@ -408,7 +408,7 @@ def test_sparse_bad_pages(cuda):
     P.check([1], [120], 8, 1, 2, 4, got, short)
 
 
-@pytest.mark.parametrize("d,kvh,block,rows,keep", [(128, 1, 128, 20, (1, 1, 14)), (128, 2, 32, 10, (2, 2, 60)), (64, 4, 16, 5, (1, 2, 61)), (256, 1, 64, 10, (1, 2, 29))])
+@pytest.mark.parametrize("d,kvh,block,rows,keep", [(128, 1, 128, 20, (1, 1, 14)), (128, 2, 32, 10, (2, 2, 60)), (64, 4, 16, 5, (1, 2, 61)), (256, 1, 64, 20, (1, 2, 29))])
 def test_sparse_many_rows_with_many_tiles_each(cuda, d, kvh, block, rows, keep):
     """Rows enough that each is one thread block's, which goes round its ring of tiles many times."""
     lens = [2900 - 37 * s for s in range(8)]
