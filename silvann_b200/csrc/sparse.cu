@@ -24,6 +24,7 @@
 #include "tensormap.cuh"
 #include <atomic>
 #include <math.h>
+#include <stddef.h>
 #include <string.h>
 
 #define SV_EXPORT extern "C" __attribute__((visibility("default")))
@@ -38,7 +39,7 @@ static constexpr int SPARSE_DEVICES = 64;
 #define SP_THREADS (SP_WARPS * 32)
 #define SP_CHUNK 4096u                        /* scores looked at in one go; the best of the chunks before them ride along */
 #define SP_CAP (SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX + 8u)
-#define SP_LIST (2u * SP_THREADS)             /* candidates among which the border is looked for: two a thread */
+#define SP_LIST 512u                          /* candidates among which the border is looked for: sixteen a lane */
 
 template <int D> struct SparseCfg {
     static constexpr int TP = D == 256 ? 32 : 64;         /* positions a tile: 16 or 32 KB of K and V */
@@ -96,43 +97,36 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
     const unsigned long long b = (unsigned long long)__double_as_longlong(s + 0.0);       /* -0 + 0 = +0: equal scores, equal keys */
     return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
-/* The nearest float of a score (which carries 2^-SHIFT), as a word that orders as floats do; NaN with minus infinity. */
+/* The nearest float of a score (which carries 2^-SHIFT), NaN with minus infinity. */
 template <int DT>
-__device__ __forceinline__ uint32_t score_word(double s) {
-    const float f = s == s ? (float)(s * __hiloint2double((Wide<DT>::SHIFT + 1023) << 20, 0)) : -INFINITY;
-    const uint32_t b = __float_as_uint(f + 0.f);
-    return (b >> 31) ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float word_float(uint32_t w) { return __uint_as_float((w >> 31) ? w & 0x7FFFFFFFu : ~w); }
-__device__ __forceinline__ uint32_t float_word(float f) { const uint32_t b = __float_as_uint(f); return (b >> 31) ? ~b : b | 0x80000000u; }
-#define SP_LOWEST 0x00800000u        /* the words of the finite floats */
-#define SP_GREATEST 0xFF7FFFFFu
+__device__ __forceinline__ float score_float(double s) { return s == s ? (float)(s * __hiloint2double((Wide<DT>::SHIFT + 1023) << 20, 0)) : -INFINITY; }
 
 /* What the ring holds before the first tile: the scores of a chunk of blocks behind the best of the chunks before, and the
  * choice's own tables. */
 struct ChoiceSmem {
-    uint32_t word[SP_CAP];                            /* a score as a float's word: tells all but the closest apart */
-    uint32_t key_hi[SP_CAP], key_lo[SP_CAP];          /* the score's 64-bit key */
+    float score[SP_CAP];                              /* to the nearest float: tells all but the closest apart; NaN where there is none */
     int32_t place[SP_CAP];                            /* the block's number in the pool, -1: none */
-    uint32_t list[SP_LIST], list_word[SP_LIST];
+    uint32_t key_hi[SP_CAP], key_lo[SP_CAP];          /* the score's 64-bit key (of the cluster's other thread blocks' shares: only once it is asked for) */
+    float list_score[SP_LIST], best[SP_THREADS];
+    uint32_t list[SP_LIST];
     uint32_t ids[SILVANN_B200_PAGED_KEEP_MAX], picked[SILVANN_B200_PAGED_KEEP_MAX];
-    uint32_t hist[256];
     double qsum[256];
-    uint32_t lo[SP_WARPS], hi[SP_WARPS], warp_in[SP_WARPS], warp_tie[SP_WARPS];
+    uint32_t warp_in[SP_WARPS], warp_tie[SP_WARPS];
     uint32_t bin, need;
+    __device__ __forceinline__ uint32_t* hist() { return (uint32_t*)best; }          /* [256], where the floats did not tell */
     __device__ __forceinline__ unsigned long long key(uint32_t i) const { return (unsigned long long)key_hi[i] << 32 | key_lo[i]; }
 };
 
 /* A histogram walked down from its top bin by one warp: the bin where the count reaches `need`, and what is still needed in it. */
 __device__ __forceinline__ void hist_walk(ChoiceSmem& S, uint32_t need, int lane) {
     uint32_t mine = 0u;
-    for (int b = 0; b < 8; ++b) mine += S.hist[255 - 8 * lane - b];
+    for (int b = 0; b < 8; ++b) mine += S.hist()[255 - 8 * lane - b];
     uint32_t upto = mine;
     for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
     const unsigned reached = __ballot_sync(0xffffffffu, upto >= need);
     if (lane == __ffs(reached) - 1) {
         uint32_t covered = upto - mine, bin = 255u - 8u * (uint32_t)lane;
-        for (int b = 0; b < 7 && covered + S.hist[bin] < need; ++b) covered += S.hist[bin--];
+        for (int b = 0; b < 7 && covered + S.hist()[bin] < need; ++b) covered += S.hist()[bin--];
         S.bin = bin; S.need = need - covered;
     }
 }
@@ -144,10 +138,10 @@ __device__ __noinline__ void choose_by_bytes(ChoiceSmem& S, uint32_t m, uint32_t
     unsigned long long known = 0ull, cut = 0ull;
     uint32_t ties = take;
     for (int shift = 56; shift >= 0; shift -= 8) {
-        S.hist[tid] = 0u;
+        S.hist()[tid] = 0u;
         __syncthreads();
         for (uint32_t i = tid; i < m; i += SP_THREADS)
-            if ((S.key(i) & known) == cut) atomicAdd(&S.hist[(uint32_t)(S.key(i) >> shift) & 255u], 1u);
+            if ((S.key(i) & known) == cut) atomicAdd(&S.hist()[(uint32_t)(S.key(i) >> shift) & 255u], 1u);
         __syncthreads();
         if (warp == 0) hist_walk(S, ties, lane);
         __syncthreads();
@@ -177,100 +171,98 @@ __device__ __noinline__ void choose_by_bytes(ChoiceSmem& S, uint32_t m, uint32_t
     __syncthreads();
 }
 
-/* A word that exactly `take` of the threads' words (K each; 0: none) reach, found by halving the interval between the least and the
- * greatest finite one with the whole block counting, a barrier a step; or 0 when there is none: equal words lie across the border, or
- * infinities do. */
+/* A number that exactly `take` of score[0..n) reach, n <= 32 K, or NaN when there is none: equal floats lie across the border,
+ * or infinities do.  The interval between the least and the greatest finite score is halved; every warp holds all scores and counts
+ * for itself, so that a step is a compare, a vote and a population count, without a barrier. */
 template <int K>
-__device__ __forceinline__ uint32_t border(ChoiceSmem& S, const uint32_t (&w)[K], uint32_t take) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t mn = 0xFFFFFFFFu, mx = 0u;
+__device__ __forceinline__ float border(const float* score, uint32_t n, uint32_t take, float (&w)[K]) {
+    const uint32_t lane = threadIdx.x & 31u;
+    float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
     for (int x = 0; x < K; ++x) {
-        if (w[x] >= SP_LOWEST && w[x] <= SP_GREATEST) { mn = min(mn, w[x]); mx = max(mx, w[x]); }
+        w[x] = x * 32u + lane < n ? score[x * 32u + lane] : __int_as_float(0x7FFFFFFF);
+        if (fabsf(w[x]) < INFINITY) { lo = fminf(lo, w[x]); hi = fmaxf(hi, w[x]); }
     }
-    mn = __reduce_min_sync(0xffffffffu, mn); mx = __reduce_max_sync(0xffffffffu, mx);
-    if (lane == 0) { S.lo[warp] = mn; S.hi[warp] = mx; }
-    __syncthreads();
 #pragma unroll
-    for (int x = 0; x < SP_WARPS; ++x) { mn = min(mn, S.lo[x]); mx = max(mx, S.hi[x]); }
-    if (mn > mx) return 0u;
-    auto reach = [&](uint32_t t) { uint32_t c = 0u;
+    for (int x = 16; x > 0; x >>= 1) { lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, x)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, x)); }
+    auto reach = [&](float t) { uint32_t c = 0u;
 #pragma unroll
-        for (int x = 0; x < K; ++x) c += __syncthreads_count(w[x] >= t);
+        for (int x = 0; x < K; ++x) c += __popc(__ballot_sync(0xffffffffu, w[x] >= t));
         return c; };
-    uint32_t c = reach(mn);
-    if (c <= take) return c == take ? mn : 0u;
-    float lo = word_float(mn), hi = word_float(mx);
+    uint32_t c = reach(lo);
+    if (c <= take) return c == take ? lo : __int_as_float(0x7FFFFFFF);
     for (int step = 0; step < 64; ++step) {
         const float mid = 0.5f * lo + 0.5f * hi;
-        if (!(mid > lo && mid < hi)) return 0u;
-        c = reach(float_word(mid));
-        if (c == take) return float_word(mid);
+        if (!(mid > lo && mid < hi)) break;
+        c = reach(mid);
+        if (c == take) return mid;
         if (c > take) lo = mid; else hi = mid;
     }
-    return 0u;
+    return __int_as_float(0x7FFFFFFF);
 }
 
-/* The `take` greatest of the m keys (equal ones: the lower index), their indexes ascending into S.picked; m > take > 0.
- * Called by SP_THREADS threads.
- * Up to 512 keys: the border between the chosen and the others is looked for among their words.  More: first among the threads' own
- * greatest words — `take` of them reach it, so at least `take` keys do, and, scores being in no order, not many more: they are
- * listed, in order, and the border looked for among them.  Where there is no border (equal words on both sides of it) or the list is
- * too long, and for more than 256 blocks, the 64-bit keys are counted a byte at a time. */
-__device__ __forceinline__ void choose(ChoiceSmem& S, uint32_t m, uint32_t take) {
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    uint32_t n = m;
-    const uint32_t* words = S.word;
-    if (m > SP_LIST) {
-        if (take > SP_THREADS) { choose_by_bytes(S, m, take); return; }
-        /* a thread's keys are neighbours, so that the list is in order */
-        constexpr int MOST = (SP_CAP + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u);        /* loads of four */
-        const uint32_t run = (m + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u) * 4u, i0 = tid * run;
-        uint32_t best[1] = {0u};
+/* The indexes of the `take` greatest of score[0..n) into S.picked, ascending, by that border (index[] of them where there is one);
+ * false when there is none.  Each warp writes its share of what all of them hold. */
+template <int K>
+__device__ __noinline__ bool choose_by_border(ChoiceSmem& S, const float* score, const uint32_t* index, uint32_t n, uint32_t take) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    float w[K];
+    const float least = border<K>(score, n, take, w);
+    if (!(least == least)) return false;
+    uint32_t at = 0u;
 #pragma unroll
-        for (int x = 0; x < MOST; ++x)
-            if (4u * x < run && i0 + 4u * x < m) { const uint4 y = *reinterpret_cast<const uint4*>(S.word + i0 + 4 * x); best[0] = max(best[0], max(max(y.x, y.y), max(y.z, y.w))); }
-        const uint32_t least = border<1>(S, best, take);
-        uint32_t hits = 0u;
-#pragma unroll
-        for (int x = 0; x < MOST; ++x)
-            if (4u * x < run && i0 + 4u * x < m) {
-                const uint4 y = *reinterpret_cast<const uint4*>(S.word + i0 + 4 * x);
-                hits |= ((y.x >= least ? 1u : 0u) | (y.y >= least ? 2u : 0u) | (y.z >= least ? 4u : 0u) | (y.w >= least ? 8u : 0u)) << (4 * x);
-            }
-        uint32_t upto = __popc(hits);
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
-        if (lane == 31u) S.warp_in[warp] = upto;
-        __syncthreads();
-        uint32_t at = upto - __popc(hits);
-        n = 0u;
-#pragma unroll
-        for (uint32_t w = 0; w < SP_WARPS; ++w) { const uint32_t c = S.warp_in[w]; if (w < warp) at += c; n += c; }
-        if (least == 0u || n > SP_LIST) { __syncthreads(); choose_by_bytes(S, m, take); return; }
-        for (; hits; hits &= hits - 1u, ++at) { const uint32_t i = i0 + __ffs(hits) - 1u; S.list[at] = i; S.list_word[at] = S.word[i]; }
-        __syncthreads();
-        words = S.list_word;
+    for (int x = 0; x < K; ++x) {
+        const unsigned in = __ballot_sync(0xffffffffu, w[x] >= least);
+        if (x % SP_WARPS == warp && w[x] >= least) S.picked[at + __popc(in & ((1u << lane) - 1u))] = index ? index[x * 32u + lane] : x * 32u + lane;
+        at += __popc(in);
     }
-    uint32_t least;
-    uint32_t w[2] = {2u * tid < n ? words[2u * tid] : 0u, 2u * tid + 1u < n ? words[2u * tid + 1u] : 0u};
-    if (n <= SP_THREADS) {
-        uint32_t one[1] = {tid < n ? words[tid] : 0u};
-        least = border<1>(S, one, take);
-        w[0] = one[0]; w[1] = 0u;
-    } else least = border<2>(S, w, take);
-    if (least == 0u) { __syncthreads(); choose_by_bytes(S, m, take); return; }
-    const bool in0 = w[0] >= least, in1 = w[1] >= least;
-    const unsigned b0 = __ballot_sync(0xffffffffu, in0), b1 = __ballot_sync(0xffffffffu, in1), below = (1u << lane) - 1u;
-    if (lane == 0u) S.warp_in[warp] = __popc(b0) + __popc(b1);
     __syncthreads();
-    uint32_t at = __popc(b0 & below) + __popc(b1 & below);
+    return true;
+}
+
+/* The `take` greatest of the m scores (equal ones: the lower index), their indexes ascending into S.picked; m > take > 0; false when the
+ * floats do not tell: the 64-bit keys have to (choose_by_bytes).  Called by SP_THREADS threads, with the same answer in all of them.
+ * Up to 512 scores: by their border.  More: first the border among the threads' own greatest — `take` of them reach it, so at least
+ * `take` scores do, and, scores being in no order, not many more: they are listed, in order, and chosen from. */
+__device__ __forceinline__ bool choose(ChoiceSmem& S, uint32_t m, uint32_t take) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    if (m <= 128u) return choose_by_border<4>(S, S.score, nullptr, m, take);
+    if (m <= 256u) return choose_by_border<8>(S, S.score, nullptr, m, take);
+    if (m <= SP_LIST) return choose_by_border<16>(S, S.score, nullptr, m, take);
+    if (take > SP_THREADS) return false;
+    /* a thread's scores are neighbours, so that the list is in order */
+    constexpr int MOST = (SP_CAP + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u);        /* loads of four */
+    const uint32_t run = (m + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u) * 4u, i0 = tid * run;
+    float best = __int_as_float(0x7FFFFFFF);
 #pragma unroll
-    for (uint32_t x = 0; x < SP_WARPS; ++x) if (x < warp) at += S.warp_in[x];
-    const uint32_t k = n <= SP_THREADS ? tid : 2u * tid;
-    if (in0) S.picked[at++] = words == S.word ? k : S.list[k];
-    if (in1) S.picked[at] = words == S.word ? k + 1u : S.list[k + 1u];
+    for (int x = 0; x < MOST; ++x)
+        if (4u * x < run && i0 + 4u * x < m) { const float4 y = *reinterpret_cast<const float4*>(S.score + i0 + 4 * x); best = fmaxf(best, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w))); }
+    S.best[tid] = best;
     __syncthreads();
+    float w[SP_THREADS / 32];
+    const float least = border<SP_THREADS / 32>(S.best, SP_THREADS, take, w);
+    if (!(least == least)) return false;
+    uint32_t hits = 0u;
+#pragma unroll
+    for (int x = 0; x < MOST; ++x)
+        if (4u * x < run && i0 + 4u * x < m) {
+            const float4 y = *reinterpret_cast<const float4*>(S.score + i0 + 4 * x);
+            hits |= ((y.x >= least ? 1u : 0u) | (y.y >= least ? 2u : 0u) | (y.z >= least ? 4u : 0u) | (y.w >= least ? 8u : 0u)) << (4 * x);
+        }
+    uint32_t upto = __popc(hits);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
+    if (lane == 31u) S.warp_in[warp] = upto;
+    __syncthreads();
+    uint32_t at = upto - __popc(hits), n = 0u;
+#pragma unroll
+    for (uint32_t x = 0; x < SP_WARPS; ++x) { const uint32_t c = S.warp_in[x]; if (x < warp) at += c; n += c; }
+    if (n > SP_LIST) return false;
+    for (; hits; hits &= hits - 1u, ++at) { const uint32_t i = i0 + __ffs(hits) - 1u; S.list[at] = i; S.list_score[at] = S.score[i]; }
+    __syncthreads();
+    if (n <= 128u) return choose_by_border<4>(S, S.list_score, S.list, n, take);
+    if (n <= 256u) return choose_by_border<8>(S, S.list_score, S.list, n, take);
+    return choose_by_border<16>(S, S.list_score, S.list, n, take);
 }
 
 /* The score of a mean that holds an infinity or a NaN (any of a warp's `count`): summed by conversion.  Such a score is no finite number
@@ -429,6 +421,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     if (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     /* ---- scores and choice, a chunk of blocks at a time ---- */
+    const bool many = c.hi - c.lo > SP_CHUNK;
     uint32_t have = 0;                                                    /* the best of the chunks so far: keys, place, ids [0..have) */
     for (uint32_t base = c.lo; c.take && base < c.hi; base += SP_CHUNK) {
         const uint32_t chunk = min(SP_CHUNK, c.hi - base), per = share(chunk), from = min(chunk, crank * per), n = min(per, chunk - from);
@@ -483,48 +476,56 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     const double score = at >= 0 ? v : -INFINITY;
                     const unsigned long long k = score_key(score);
                     const uint32_t z = front + from + i;
-                    S.word[z] = score_word<DT>(score); S.key_hi[z] = (uint32_t)(k >> 32); S.key_lo[z] = (uint32_t)k; S.place[z] = at;
+                    S.score[z] = score_float<DT>(score); S.key_hi[z] = (uint32_t)(k >> 32); S.key_lo[z] = (uint32_t)k; S.place[z] = at;
                 }
             }
         }
-        /* between the best of the chunks before and this chunk, and behind it: words and keys that no score has */
+        /* between the best of the chunks before and this chunk, and behind it: no scores, and keys that none has */
         if (tid < 4u) {
-            if (have + tid < front) { S.word[have + tid] = 0u; S.key_hi[have + tid] = 0u; S.key_lo[have + tid] = 0u; }
-            S.word[front + chunk + tid] = 0u; S.key_hi[front + chunk + tid] = 0u; S.key_lo[front + chunk + tid] = 0u;
+            if (have + tid < front) { S.score[have + tid] = __int_as_float(0x7FFFFFFF); S.key_hi[have + tid] = 0u; S.key_lo[have + tid] = 0u; }
+            S.score[front + chunk + tid] = __int_as_float(0x7FFFFFFF); S.key_hi[front + chunk + tid] = 0u; S.key_lo[front + chunk + tid] = 0u;
         }
-        if (CL > 1) {
-            __syncthreads();
-            /* this block's scores to every peer (what lies behind the chunk's last is zeros there as well) */
-            const uint32_t quads = (n + 3u) / 4u;
-            for (uint32_t z = tid; z < quads * 4u * CL; z += SP_THREADS) {
-                const uint32_t to = z / (quads * 4u), a = z / quads % 4u, at = front + from + z % quads * 4u;
-                const uint32_t* src = a == 0u ? S.word : a == 1u ? S.key_hi : a == 2u ? S.key_lo : (const uint32_t*)S.place;
-                if (to == crank) continue;
-                const uint4 y = *reinterpret_cast<const uint4*>(src + at);
-                asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(peer_addr(src + at, to)), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+        /* this thread block's share of two arrays to every peer, four entries at a time (behind the chunk's last there is the same everywhere) */
+        auto send = [&](const uint32_t* two) {
+            for (uint32_t z = tid >> 1; z < (n + 3u) / 4u; z += SP_THREADS / 2u) {
+                const uint32_t* src = two + (tid & 1u) * SP_CAP + front + from + z * 4u;
+                const uint4 y = *reinterpret_cast<const uint4*>(src);
+#pragma unroll 4
+                for (uint32_t to = 0; to < CL; ++to)
+                    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(peer_addr(src, to)), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
             }
+        };
+        __syncthreads();
+        if (CL > 1) {
+            send((const uint32_t*)S.score);
+            if (many) send(S.key_hi);                                     /* the best go on to the next chunk with their keys */
             cluster_sync_all();
-        } else __syncthreads();
+        }
         const uint32_t m = front + chunk;
         const bool more = base + SP_CHUNK < c.hi;
         /* (a chunk holds more blocks than can be chosen, or all there are: m > take) */
-        choose(S, m, c.take);
+        if (!choose(S, m, c.take)) {                                      /* all of the cluster's thread blocks come by here, or none */
+            __syncthreads();
+            if (CL > 1 && !many) { send(S.key_hi); cluster_sync_all(); }
+            choose_by_bytes(S, m, c.take);
+        }
         auto id_of = [&](uint32_t i) { return i < have ? S.ids[i] : base + (i - front); };
         if (more) {
             /* the chosen move to the front, in order: read all, then write */
             constexpr int KP = SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS;
-            uint32_t kw[KP], kh[KP], kl[KP], ii[KP];
+            float ks[KP];
+            uint32_t kh[KP], kl[KP], ii[KP];
             int32_t pp[KP];
 #pragma unroll
             for (int z = 0; z < KP; ++z) {
                 const uint32_t i = tid + z * SP_THREADS;
-                if (i < c.take) { const uint32_t at = S.picked[i]; kw[z] = S.word[at]; kh[z] = S.key_hi[at]; kl[z] = S.key_lo[at]; ii[z] = id_of(at); pp[z] = S.place[at]; }
+                if (i < c.take) { const uint32_t at = S.picked[i]; ks[z] = S.score[at]; kh[z] = S.key_hi[at]; kl[z] = S.key_lo[at]; ii[z] = id_of(at); pp[z] = S.place[at]; }
             }
             __syncthreads();
 #pragma unroll
             for (int z = 0; z < KP; ++z) {
                 const uint32_t i = tid + z * SP_THREADS;
-                if (i < c.take) { S.word[i] = kw[z]; S.key_hi[i] = kh[z]; S.key_lo[i] = kl[z]; S.ids[i] = ii[z]; S.place[i] = pp[z]; }
+                if (i < c.take) { S.score[i] = ks[z]; S.key_hi[i] = kh[z]; S.key_lo[i] = kl[z]; S.ids[i] = ii[z]; S.place[i] = pp[z]; }
             }
             have = c.take;
             /* no one writes the next scores over what a peer still reads */
@@ -796,6 +797,7 @@ static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& v
     constexpr size_t fixed = 1024 + (size_t)Cfg::STAGES * Cfg::STAGE_BYTES + Cfg::BOXES * 8 * NHT * 128 + 8 * NHT * (D + 32) * 4 + (2 * Cfg::STAGES + 1) * 8;
     const size_t smem = fixed + (size_t)keep * 4;
     static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= sizeof(ChoiceSmem), "the scores fit the ring");
+    static_assert(offsetof(ChoiceSmem, place) == SP_CAP * 4 && offsetof(ChoiceSmem, key_lo) == offsetof(ChoiceSmem, key_hi) + SP_CAP * 4, "arrays that are sent lie in pairs");
     static_assert(fixed + SILVANN_B200_PAGED_KEEP_MAX * 4 <= 227 * 1024, "a thread block's shared memory");
     static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (size_t)Cfg::PW * 8 * NHT * (D + 6) * 4, "the partials fit the ring");
     static std::atomic<bool> attr_set[SPARSE_DEVICES];
