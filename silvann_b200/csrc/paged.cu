@@ -18,7 +18,8 @@ namespace sv {
 /* ---------------------------------------------------------------------------------------------------------- */
 /* the step's tables                                                                                            */
 
-#define SV_TABLES_THREADS 1024
+#define SV_TABLES_THREADS 512
+#define SV_TABLES_CLUSTER 8u
 static constexpr int TABLES_DEVICES = 64;
 
 struct TablesParams {
@@ -28,118 +29,146 @@ struct TablesParams {
     const uint32_t* free_at;
     const int32_t *lens, *counts;
     unsigned int* status;
-    uint32_t seqs, stride, rows, free_total, pool_pages, page_pos;
+    PagedDiv page;                      /* positions a page */
+    uint64_t most;                      /* positions a table row has pages for */
+    uint32_t seqs, stride, rows, free_total, pool_pages;
 };
 
 /* What one sequence brings to the three sums: new positions, pages it takes, pages it gives back. */
 struct TablesItem { uint32_t rows, need, back; bool bad; };
+__device__ __forceinline__ uint32_t tables_pages(const TablesParams& P, uint32_t n) { return n ? paged_quot(n - 1u, P.page) + 1u : 0u; }
 __device__ __forceinline__ TablesItem tables_item(const TablesParams& P, int32_t len, int32_t count) {
     TablesItem it = {0u, 0u, 0u, false};
-    const uint64_t most = (uint64_t)P.stride * P.page_pos;
-    if (len < 0 || count < SILVANN_B200_PAGED_ENDED || (uint64_t)len + (uint64_t)(count > 0 ? count : 0) > most ||
-        (int64_t)len + (count > 0 ? count : 0) > 0x7FFFFFFFll) { it.bad = true; return it; }
-    const uint32_t held = ((uint32_t)len + P.page_pos - 1u) / P.page_pos;
+    const uint32_t come = count > 0 ? (uint32_t)count : 0u;
+    if (len < 0 || count < SILVANN_B200_PAGED_ENDED || (uint64_t)len + come > P.most || (uint64_t)len + come > 0x7FFFFFFFull) { it.bad = true; return it; }
+    const uint32_t held = tables_pages(P, (uint32_t)len);
     if (count < 0) it.back = held;
-    else { it.rows = (uint32_t)count; it.need = ((uint32_t)len + (uint32_t)count + P.page_pos - 1u) / P.page_pos - held; }
+    else { it.rows = come; it.need = tables_pages(P, (uint32_t)len + come) - held; }
     return it;
 }
+/* Sums stop at 2^32 - 1, beyond every size they are compared with. */
+__device__ __forceinline__ uint32_t tables_add(uint32_t a, uint32_t b) { const uint32_t c = a + b; return c < a ? 0xFFFFFFFFu : c; }
 
-/* The sequence that item j of a list belongs to: the last s with start[s] <= j among those that have items. */
-__device__ __forceinline__ uint32_t tables_owner(const uint32_t* start, uint32_t seqs, uint32_t j) {
-    uint32_t lo = 0u, hi = seqs;                       /* start[lo] <= j < start[hi] */
+/* The sequence that item j of a list belongs to, looked for in [lo, hi]: the last s with start[s] <= j among those that have items. */
+__device__ __forceinline__ uint32_t tables_owner(const uint32_t* start, uint32_t lo, uint32_t hi, uint32_t j) {
+    ++hi;                                              /* start[lo] <= j < start[hi] */
     while (hi - lo > 1u) { const uint32_t mid = (lo + hi) >> 1; if (start[mid] <= j) lo = mid; else hi = mid; }
     return lo;
 }
 
-/* Exclusive sums of (rows, need, back) over the sequences, then three flat lists — pages that come back, pages handed out,
- * new positions — walked by all threads.  The whole step is decided (fits or is refused) before anything is written. */
+/* Every thread block of the one cluster makes the exclusive sums of (rows, need, back) over all sequences for itself, in its own shared
+ * memory: the step is decided (it fits or is refused) before anything is written, without an exchange.  Then three flat lists — pages
+ * that come back, pages handed out, new positions — are walked by all threads of the cluster.  One barrier of the cluster stands between
+ * what reads the caller's arrays and what may write them in place, and between the pages that come back and those handed out.
+ * A step is a handful of dependent reads long; the cluster is there for the steps that bring many positions. */
 __global__ void __launch_bounds__(SV_TABLES_THREADS, 1) paged_tables_kernel(const TablesParams P) {
     extern __shared__ uint32_t tsm[];
     uint32_t* rows_s = tsm;                       /* [seqs + 1] each */
     uint32_t* need_s = rows_s + P.seqs + 1;
     uint32_t* back_s = need_s + P.seqs + 1;
     int32_t* len_s = (int32_t*)(back_s + P.seqs + 1);
-    __shared__ unsigned long long warp_sum[3][32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t per = (P.seqs + SV_TABLES_THREADS - 1) / SV_TABLES_THREADS;
+    constexpr uint32_t WARPS = SV_TABLES_THREADS / 32;
+    __shared__ uint32_t warp_sum[3][WARPS];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t CL = cluster_nctarank(), g_tid = cluster_ctarank() * SV_TABLES_THREADS + tid, g_all = CL * SV_TABLES_THREADS;
+    const uint32_t per = (P.seqs + SV_TABLES_THREADS - 1u) / SV_TABLES_THREADS;
     const uint32_t i0 = min(P.seqs, tid * per), i1 = min(P.seqs, i0 + per);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t at = *P.free_at;
 
-    unsigned long long sum[3] = {0, 0, 0};
+    uint32_t sum[3] = {0u, 0u, 0u};
     bool bad = false;
+    const int32_t len0 = i0 < i1 ? P.lens[i0] : 0, count0 = i0 < i1 ? P.counts[i0] : 0;
     for (uint32_t s = i0; s < i1; ++s) {
-        const TablesItem it = tables_item(P, P.lens[s], P.counts[s]);
-        sum[0] += it.rows; sum[1] += it.need; sum[2] += it.back; bad |= it.bad;
+        const int32_t len = s == i0 ? len0 : P.lens[s];
+        const TablesItem it = tables_item(P, len, s == i0 ? count0 : P.counts[s]);
+        rows_s[s] = sum[0]; need_s[s] = sum[1]; back_s[s] = sum[2]; len_s[s] = len;      /* up to here within this thread */
+        sum[0] = tables_add(sum[0], it.rows); sum[1] = tables_add(sum[1], it.need); sum[2] = tables_add(sum[2], it.back); bad |= it.bad;
     }
-    unsigned long long before[3];
+    uint32_t before[3], all[3] = {0u, 0u, 0u};
 #pragma unroll
     for (int x = 0; x < 3; ++x) {
-        unsigned long long v = sum[x];
-        for (int d = 1; d < 32; d <<= 1) { const unsigned long long o = __shfl_up_sync(0xffffffffu, v, d); if (lane >= d) v += o; }
-        if (lane == 31) warp_sum[x][warp] = v;
-        before[x] = v - sum[x];
+        uint32_t v = sum[x];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, v, d); if (lane >= d) v = tables_add(v, o); }
+        if (lane == 31u) warp_sum[x][warp] = v;
+        before[x] = __shfl_up_sync(0xffffffffu, v, 1);
+        if (lane == 0u) before[x] = 0u;
     }
     bad = __syncthreads_or(bad);
-    unsigned long long all[3];
 #pragma unroll
-    for (int x = 0; x < 3; ++x) {
-        unsigned long long w = 0, mine = 0;
-        for (int u = 0; u < 32; ++u) { if (u == warp) mine = w; w += warp_sum[x][u]; }
-        before[x] += mine; all[x] = w;
-    }
+    for (uint32_t u = 0; u < WARPS; ++u)
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+            const uint32_t w = warp_sum[x][u];
+            if (u < warp) before[x] = tables_add(before[x], w);
+            all[x] = tables_add(all[x], w);
+        }
     const bool bad_step = bad || all[0] > P.rows || at > P.free_total || all[2] > at;
-    const bool no_pages = !bad_step && all[1] > (unsigned long long)P.free_total - (at - all[2]);
+    const bool no_pages = !bad_step && all[1] > P.free_total - (at - all[2]);
 
     if (bad_step || no_pages) {
-        if (tid == 0) {
+        __syncthreads();
+        if (CL > 1) cluster_sync_all();
+        if (g_tid == 0) {
             if (P.status) atomicOr(P.status, bad_step ? SV_STATUS_BAD_STEP : SV_STATUS_NO_PAGES);
             *P.free_out = at;
         }
-        for (uint32_t s = tid; s <= P.seqs; s += blockDim.x) { if (s < P.seqs) P.new_lens[s] = P.lens[s]; P.row_start[s] = 0; }
-        for (uint32_t r = tid; r < P.rows; r += blockDim.x) { P.row_seq[r] = -1; P.row_pos[r] = -1; P.row_slot[r] = -1; }
+        for (uint32_t s = g_tid; s <= P.seqs; s += g_all) { if (s < P.seqs) P.new_lens[s] = len_s[s]; P.row_start[s] = 0; }
+        for (uint32_t r = g_tid; r < P.rows; r += g_all) { P.row_seq[r] = -1; P.row_pos[r] = -1; P.row_slot[r] = -1; }
         return;
     }
-    for (uint32_t s = i0; s < i1; ++s) {
-        const int32_t len = P.lens[s];
-        const TablesItem it = tables_item(P, len, P.counts[s]);
-        rows_s[s] = (uint32_t)before[0]; need_s[s] = (uint32_t)before[1]; back_s[s] = (uint32_t)before[2]; len_s[s] = len;
-        before[0] += it.rows; before[1] += it.need; before[2] += it.back;
-    }
-    if (tid == 0) { rows_s[P.seqs] = (uint32_t)all[0]; need_s[P.seqs] = (uint32_t)all[1]; back_s[P.seqs] = (uint32_t)all[2]; }
+    for (uint32_t s = i0; s < i1; ++s) { rows_s[s] += before[0]; need_s[s] += before[1]; back_s[s] += before[2]; }
+    if (tid == 0) { rows_s[P.seqs] = all[0]; need_s[P.seqs] = all[1]; back_s[P.seqs] = all[2]; }
     __syncthreads();
-    const uint32_t n_rows = (uint32_t)all[0], n_need = (uint32_t)all[1], n_back = (uint32_t)all[2], bottom = at - n_back;
+    const uint32_t n_rows = all[0], n_need = all[1], n_back = all[2], bottom = at - n_back, last = P.seqs - 1u;
     bool strange = false;                          /* an entry that names no page of the pool */
 
-    for (uint32_t j = tid; j < n_back; j += blockDim.x) {
-        const uint32_t s = tables_owner(back_s, P.seqs, j);
+    for (uint32_t j = g_tid; j < n_back; j += g_all) {
+        const uint32_t s = tables_owner(back_s, 0u, last, j);
         const int32_t page = P.table[(size_t)s * P.stride + (j - back_s[s])];
         strange |= page < 0 || (uint32_t)page >= P.pool_pages;
         P.free_pages[bottom + j] = page;
     }
-    __syncthreads();
-    for (uint32_t s = tid; s <= P.seqs; s += blockDim.x) {
+    if (CL > 1) cluster_sync_all(); else __syncthreads();
+    for (uint32_t s = g_tid; s <= P.seqs; s += g_all) {
         P.row_start[s] = (int32_t)rows_s[s];
         if (s < P.seqs) P.new_lens[s] = back_s[s + 1] > back_s[s] ? 0 : len_s[s] + (int32_t)(rows_s[s + 1] - rows_s[s]);
     }
-    if (tid == 0) *P.free_out = bottom + n_need;
-    for (uint32_t j = tid; j < n_need; j += blockDim.x) {
-        const uint32_t s = tables_owner(need_s, P.seqs, j);
-        const int32_t page = P.free_pages[bottom + j];
+    if (g_tid == 0) *P.free_out = bottom + n_need;
+    for (uint32_t j = g_tid; j < n_need; j += g_all) {
+        const uint32_t s = tables_owner(need_s, 0u, last, j);
+        const int32_t page = __ldcg(P.free_pages + bottom + j);
         strange |= page < 0 || (uint32_t)page >= P.pool_pages;
-        P.table[(size_t)s * P.stride + ((uint32_t)len_s[s] + P.page_pos - 1u) / P.page_pos + (j - need_s[s])] = page;
+        P.table[(size_t)s * P.stride + tables_pages(P, (uint32_t)len_s[s]) + (j - need_s[s])] = page;
     }
-    for (uint32_t r = tid; r < P.rows; r += blockDim.x) {
-        int32_t seq = -1, pos = -1, slot = -1;
-        if (r < n_rows) {
-            const uint32_t s = tables_owner(rows_s, P.seqs, r);
-            const uint32_t len = (uint32_t)len_s[s], p = len + (r - rows_s[s]), col = p / P.page_pos, held = (len + P.page_pos - 1u) / P.page_pos;
-            /* a page taken in this step is read from the stack, where it came from */
-            const int32_t page = col < held ? P.table[(size_t)s * P.stride + col] : P.free_pages[bottom + need_s[s] + (col - held)];
-            seq = (int32_t)s; pos = (int32_t)p;
-            if (page < 0 || (uint32_t)page >= P.pool_pages) strange = true;
-            else slot = (int32_t)((uint32_t)page * P.page_pos + (p - col * P.page_pos));
+    /* a warp takes 128 neighbouring rows: four a lane, their pages asked for together; the sequences of the warp's first and last row
+     * bound where the others are looked for */
+    constexpr uint32_t U = 4;
+    for (uint32_t r0 = (g_tid & ~31u) * U; r0 < P.rows; r0 += g_all * U) {
+        uint32_t s_lo = 0u, s_hi = 0u;
+        if (r0 < n_rows) { s_lo = tables_owner(rows_s, 0u, last, r0); s_hi = tables_owner(rows_s, s_lo, last, min(r0 + 32u * U, n_rows) - 1u); }
+        int32_t seq[U], pos[U], page[U];
+        uint32_t off[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t r = r0 + u * 32u + lane;
+            seq[u] = pos[u] = page[u] = -1; off[u] = 0u;
+            if (r < n_rows) {
+                const uint32_t s = s_lo == s_hi ? s_lo : tables_owner(rows_s, s_lo, s_hi, r);
+                const uint32_t len = (uint32_t)len_s[s], p = len + (r - rows_s[s]), col = paged_quot(p, P.page), held = tables_pages(P, len);
+                seq[u] = (int32_t)s; pos[u] = (int32_t)p; off[u] = p - col * P.page.d;
+                /* a page taken in this step is read from the stack, where it came from */
+                page[u] = col < held ? P.table[(size_t)s * P.stride + col] : __ldcg(P.free_pages + bottom + need_s[s] + (col - held));
+                if (page[u] < 0 || (uint32_t)page[u] >= P.pool_pages) { strange = true; page[u] = -1; }
+            }
         }
-        P.row_seq[r] = seq; P.row_pos[r] = pos; P.row_slot[r] = slot;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t r = r0 + u * 32u + lane;
+            if (r < P.rows) { P.row_seq[r] = seq[u]; P.row_pos[r] = pos[u]; P.row_slot[r] = page[u] < 0 ? -1 : (int32_t)((uint32_t)page[u] * P.page.d + off[u]); }
+        }
     }
     if (strange && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE);
 }
@@ -153,7 +182,17 @@ static cudaError_t tables_launch(const TablesParams& P, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         attr_set[d].store(true, std::memory_order_release);
     }
-    paged_tables_kernel<<<1, SV_TABLES_THREADS, smem, st>>>(P);
+    /* one thread block takes four rows a thread in a round; a cluster where there are more */
+    const uint32_t cluster = P.rows <= 4u * SV_TABLES_THREADS ? 1u : SV_TABLES_CLUSTER;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster); cfg.blockDim = dim3(SV_TABLES_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    unsigned na = 0;
+    if (cluster > 1u) { attr[na].id = cudaLaunchAttributeClusterDimension; attr[na].val.clusterDim.x = cluster; attr[na].val.clusterDim.y = 1; attr[na].val.clusterDim.z = 1; ++na; }
+    if (pdl_allowed()) { attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[na].val.programmaticStreamSerializationAllowed = 1; ++na; }
+    cfg.attrs = attr; cfg.numAttrs = na;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, paged_tables_kernel, P);
+    if (e != cudaSuccess) return e;
     note_launch(1);
     return cudaGetLastError();
 }
@@ -224,7 +263,8 @@ SV_EXPORT int silvann_b200_paged_tables(int32_t* new_lens, int32_t* page_table, 
     sv::TablesParams P;
     P.new_lens = new_lens; P.table = page_table; P.row_start = row_start; P.row_seq = row_seq; P.row_pos = row_pos; P.row_slot = row_slot;
     P.free_out = free_out; P.free_pages = free_pages; P.free_at = free_at; P.lens = lens; P.counts = counts; P.status = sv::device_status_word();
-    P.seqs = seqs; P.stride = table_stride; P.rows = rows; P.free_total = free_total; P.pool_pages = (uint32_t)pool_pages; P.page_pos = page_positions;
+    P.seqs = seqs; P.stride = table_stride; P.rows = rows; P.free_total = free_total; P.pool_pages = (uint32_t)pool_pages; P.page = sv::paged_div(page_positions);
+    P.most = (uint64_t)table_stride * page_positions;
     cudaError_t e = sv::tables_launch(P, (cudaStream_t)stream);
     return e == cudaSuccess ? SILVANN_B200_OK : cuda_fail("paged_tables: launch", e);
 }
