@@ -414,7 +414,8 @@ int silvann_b200_paged_tables(int32_t* new_lens, int32_t* page_table, int32_t* r
  * SILVANN_B200_STATUS_BAD_PAGE.  k_stride and v_stride are the elements from one row to the next (0: packed), so that rows
  * may be read out of a wider projection.  With block_positions B (16, 32, 64 or 128, a divisor of page_positions; 0: k_means
  * is not touched) a row that is the last of a block, slot % B == B - 1, also leaves the block's mean key at
- * k_means[slot / B][kv_heads][head_dim]: the fp32 sum of the block's B rows in ascending order, over B, rounded to `dtype`.
+ * k_means[slot / B][kv_heads][head_dim]: the fp32 sum of the block's B rows, sixteen in ascending order and those sums in
+ * ascending order, over B, rounded to `dtype`.
  * Rows of one block must stand in ascending order next to each other (as paged_tables numbers them), earlier ones in the
  * pool; no slot may be named twice.  kv_heads * head_dim and the strides are multiples of 8, addresses of 16 bytes. */
 int silvann_b200_paged_write(void* k_pool, void* v_pool, void* k_means, const void* k_rows, const void* v_rows, uint64_t k_stride,
