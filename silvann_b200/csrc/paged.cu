@@ -49,11 +49,64 @@ __device__ __forceinline__ TablesItem tables_item(const TablesParams& P, int32_t
 /* Sums stop at 2^32 - 1, beyond every size they are compared with. */
 __device__ __forceinline__ uint32_t tables_add(uint32_t a, uint32_t b) { const uint32_t c = a + b; return c < a ? 0xFFFFFFFFu : c; }
 
-/* The sequence that item j of a list belongs to, looked for in [lo, hi]: the last s with start[s] <= j among those that have items. */
-__device__ __forceinline__ uint32_t tables_owner(const uint32_t* start, uint32_t lo, uint32_t hi, uint32_t j) {
-    ++hi;                                              /* start[lo] <= j < start[hi] */
-    while (hi - lo > 1u) { const uint32_t mid = (lo + hi) >> 1; if (start[mid] <= j) lo = mid; else hi = mid; }
-    return lo;
+/* The sequences that N items of a list belong to, each looked for among `n` from `lo` on: the last s with start[s] <= item among those
+ * that have items.  The N searches go hand in hand. */
+template <int N>
+__device__ __forceinline__ void tables_owners(const uint32_t* start, uint32_t lo, uint32_t n, const uint32_t (&item)[N], uint32_t (&s)[N]) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) s[u] = lo;
+    while (n > 1u) {
+        const uint32_t half = n >> 1;
+#pragma unroll
+        for (int u = 0; u < N; ++u) if (start[s[u] + half] <= item[u]) s[u] += half;
+        n -= half;
+    }
+}
+__device__ __forceinline__ uint32_t tables_owner(const uint32_t* start, uint32_t lo, uint32_t n, uint32_t item) {
+    const uint32_t i[1] = {item};
+    uint32_t s[1];
+    tables_owners<1>(start, lo, n, i, s);
+    return s[0];
+}
+
+/* New positions, U of them a lane: a warp takes 32 U neighbouring ones, whose sequences lie between those of its first and its last. */
+template <int U>
+__device__ __forceinline__ bool tables_rows(const TablesParams& P, const uint32_t* rows_s, const uint32_t* need_s, const int32_t* len_s, uint32_t n_rows, uint32_t bottom,
+                                            uint32_t g_tid, uint32_t g_all) {
+    const uint32_t lane = g_tid & 31u;
+    bool strange = false;
+    for (uint32_t r0 = (g_tid & ~31u) * U; r0 < P.rows; r0 += g_all * U) {
+        uint32_t s_lo = 0u, span = 1u;
+        if (r0 < n_rows) {
+            const uint32_t ends[2] = {r0, min(r0 + 32u * U, n_rows) - 1u};
+            uint32_t s[2];
+            tables_owners<2>(rows_s, 0u, P.seqs, ends, s);
+            s_lo = s[0]; span = s[1] - s[0] + 1u;
+        }
+        uint32_t row[U], s[U], off[U];
+        int32_t pos[U], page[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) row[u] = r0 + u * 32u + lane;
+        tables_owners<U>(rows_s, s_lo, span, row, s);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            page[u] = -1; off[u] = 0u; pos[u] = -1;
+            if (row[u] < n_rows) {
+                const uint32_t len = (uint32_t)len_s[s[u]], p = len + (row[u] - rows_s[s[u]]), col = paged_quot(p, P.page), held = tables_pages(P, len);
+                pos[u] = (int32_t)p; off[u] = p - col * P.page.d;
+                /* a page taken in this step is read from the stack, where it came from */
+                page[u] = col < held ? P.table[(size_t)s[u] * P.stride + col] : __ldcg(P.free_pages + bottom + need_s[s[u]] + (col - held));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (row[u] < P.rows) {
+                const bool there = row[u] < n_rows, good = page[u] >= 0 && (uint32_t)page[u] < P.pool_pages;
+                strange |= there && !good;
+                P.row_seq[row[u]] = there ? (int32_t)s[u] : -1; P.row_pos[row[u]] = pos[u]; P.row_slot[row[u]] = good ? (int32_t)((uint32_t)page[u] * P.page.d + off[u]) : -1;
+            }
+    }
+    return strange;
 }
 
 /* Every thread block of the one cluster makes the exclusive sums of (rows, need, back) over all sequences for itself, in its own shared
@@ -86,7 +139,7 @@ __global__ void __launch_bounds__(SV_TABLES_THREADS, 1) paged_tables_kernel(cons
         rows_s[s] = sum[0]; need_s[s] = sum[1]; back_s[s] = sum[2];                     /* up to here within this thread */
         sum[0] = tables_add(sum[0], it.rows); sum[1] = tables_add(sum[1], it.need); sum[2] = tables_add(sum[2], it.back); bad |= it.bad;
     }
-    uint32_t before[3], all[3] = {0u, 0u, 0u};
+    uint32_t before[3], all[3];
 #pragma unroll
     for (int x = 0; x < 3; ++x) {
         uint32_t v = sum[x];
@@ -97,14 +150,16 @@ __global__ void __launch_bounds__(SV_TABLES_THREADS, 1) paged_tables_kernel(cons
         if (lane == 0u) before[x] = 0u;
     }
     bad = __syncthreads_or(bad);
-#pragma unroll 4
-    for (uint32_t u = 0; u < threads / 32u; ++u)
+    /* every warp sums the warps' totals for itself */
 #pragma unroll
-        for (int x = 0; x < 3; ++x) {
-            const uint32_t w = warp_sum[x][u];
-            if (u < warp) before[x] = tables_add(before[x], w);
-            all[x] = tables_add(all[x], w);
-        }
+    for (int x = 0; x < 3; ++x) {
+        uint32_t v = lane < threads / 32u ? warp_sum[x][lane] : 0u;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, v, d); if (lane >= d) v = tables_add(v, o); }
+        const uint32_t ahead = __shfl_sync(0xffffffffu, v, (warp + 31u) & 31u);
+        if (warp) before[x] = tables_add(before[x], ahead);
+        all[x] = __shfl_sync(0xffffffffu, v, 31);
+    }
     const bool bad_step = bad || all[0] > P.rows || at > P.free_total || all[2] > at;
     const bool no_pages = !bad_step && all[1] > P.free_total - (at - all[2]);
 
@@ -122,11 +177,11 @@ __global__ void __launch_bounds__(SV_TABLES_THREADS, 1) paged_tables_kernel(cons
     for (uint32_t s = i0; s < i1; ++s) { rows_s[s] += before[0]; need_s[s] += before[1]; back_s[s] += before[2]; }
     if (tid == 0) { rows_s[P.seqs] = all[0]; need_s[P.seqs] = all[1]; back_s[P.seqs] = all[2]; }
     __syncthreads();
-    const uint32_t n_rows = all[0], n_need = all[1], n_back = all[2], bottom = at - n_back, last = P.seqs - 1u;
+    const uint32_t n_rows = all[0], n_need = all[1], n_back = all[2], bottom = at - n_back;
     bool strange = false;                          /* an entry that names no page of the pool */
 
     for (uint32_t j = g_tid; j < n_back; j += g_all) {
-        const uint32_t s = tables_owner(back_s, 0u, last, j);
+        const uint32_t s = tables_owner(back_s, 0u, P.seqs, j);
         const int32_t page = P.table[(size_t)s * P.stride + (j - back_s[s])];
         strange |= page < 0 || (uint32_t)page >= P.pool_pages;
         P.free_pages[bottom + j] = page;
@@ -138,38 +193,12 @@ __global__ void __launch_bounds__(SV_TABLES_THREADS, 1) paged_tables_kernel(cons
     }
     if (g_tid == 0) *P.free_out = bottom + n_need;
     for (uint32_t j = g_tid; j < n_need; j += g_all) {
-        const uint32_t s = tables_owner(need_s, 0u, last, j);
+        const uint32_t s = tables_owner(need_s, 0u, P.seqs, j);
         const int32_t page = __ldcg(P.free_pages + bottom + j);
         strange |= page < 0 || (uint32_t)page >= P.pool_pages;
         P.table[(size_t)s * P.stride + tables_pages(P, (uint32_t)len_s[s]) + (j - need_s[s])] = page;
     }
-    /* a warp takes 128 neighbouring rows: four a lane, their pages asked for together; the sequences of the warp's first and last row
-     * bound where the others are looked for */
-    constexpr uint32_t U = 4;
-    for (uint32_t r0 = (g_tid & ~31u) * U; r0 < P.rows; r0 += g_all * U) {
-        uint32_t s_lo = 0u, s_hi = 0u;
-        if (r0 < n_rows) { s_lo = tables_owner(rows_s, 0u, last, r0); s_hi = tables_owner(rows_s, s_lo, last, min(r0 + 32u * U, n_rows) - 1u); }
-        int32_t seq[U], pos[U], page[U];
-        uint32_t off[U];
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t r = r0 + u * 32u + lane;
-            seq[u] = pos[u] = page[u] = -1; off[u] = 0u;
-            if (r < n_rows) {
-                const uint32_t s = s_lo == s_hi ? s_lo : tables_owner(rows_s, s_lo, s_hi, r);
-                const uint32_t len = (uint32_t)len_s[s], p = len + (r - rows_s[s]), col = paged_quot(p, P.page), held = tables_pages(P, len);
-                seq[u] = (int32_t)s; pos[u] = (int32_t)p; off[u] = p - col * P.page.d;
-                /* a page taken in this step is read from the stack, where it came from */
-                page[u] = col < held ? P.table[(size_t)s * P.stride + col] : __ldcg(P.free_pages + bottom + need_s[s] + (col - held));
-                if (page[u] < 0 || (uint32_t)page[u] >= P.pool_pages) { strange = true; page[u] = -1; }
-            }
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t r = r0 + u * 32u + lane;
-            if (r < P.rows) { P.row_seq[r] = seq[u]; P.row_pos[r] = pos[u]; P.row_slot[r] = page[u] < 0 ? -1 : (int32_t)((uint32_t)page[u] * P.page.d + off[u]); }
-        }
-    }
+    strange |= P.rows <= g_all ? tables_rows<1>(P, rows_s, need_s, len_s, n_rows, bottom, g_tid, g_all) : tables_rows<4>(P, rows_s, need_s, len_s, n_rows, bottom, g_tid, g_all);
     if (strange && P.status) atomicOr(P.status, SV_STATUS_BAD_PAGE);
 }
 
