@@ -42,13 +42,14 @@ static constexpr int SPARSE_DEVICES = 64;
 #define SP_LIST 512u                          /* candidates among which the border is looked for: sixteen a lane */
 
 template <int D> struct SparseCfg {
-    static constexpr int TP = D == 256 ? 32 : 64;         /* positions a tile: 16 or 32 KB of K and V */
+    static constexpr int TP = D == 256 ? 32 : D == 128 ? 64 : 128;         /* positions a tile: 32 KB of K and V */
     static constexpr int PW = TP / 16;                    /* warps that share a tile by positions; SP_WARPS / PW share it by value columns */
     static constexpr int BOXES = D / 64;                  /* 64-column (128-byte) boxes a row */
     static constexpr int BOX_BYTES = TP * 128;
     static constexpr int K_BYTES = BOXES * BOX_BYTES;
     static constexpr int STAGE_BYTES = 2 * K_BYTES;       /* K then V */
-    static constexpr int STAGES = D == 64 ? 6 : 3;        /* 96 KB: two thread blocks an SM */
+    static constexpr int STAGES = D == 64 ? 2 : 3;        /* 96 KB, two thread blocks an SM; at 64 64 KB, three */
+    static constexpr int OCC = D == 64 ? 3 : 2;
     /* scores: lanes a mean, 16-byte pieces of it a lane, means a warp takes in a round, rounds asked for at once */
     static constexpr int LPB = D == 256 ? 16 : 8;
     static constexpr int CPL = D / 8 / LPB;
@@ -67,6 +68,7 @@ struct SparseParams {
     uint64_t q_stride;
     PagedDiv per;                       /* blocks a page */
     uint32_t seqs, stride, pool_pages, page_pos, block, q_heads, kv_heads, group, head_blocks, first, last, top;
+    uint32_t chunk, cap, choice_top, ring_bytes;      /* scores looked at in one go, and room for them; the ring, or what lies in its place before */
     float scale_log2;
     bool o_wide;                        /* o starts on 8 bytes */
 };
@@ -101,24 +103,31 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 template <int DT>
 __device__ __forceinline__ float score_float(double s) { return s == s ? (float)(s * __hiloint2double((Wide<DT>::SHIFT + 1023) << 20, 0)) : -INFINITY; }
 
-/* What the ring holds before the first tile: the scores of a chunk of blocks behind the best of the chunks before, and the
- * choice's own tables. */
-struct ChoiceSmem {
-    float score[SP_CAP];                              /* to the nearest float: tells all but the closest apart; NaN where there is none */
-    int32_t place[SP_CAP];                            /* the block's number in the pool, -1: none */
-    uint32_t key_hi[SP_CAP], key_lo[SP_CAP];          /* the score's 64-bit key (of the cluster's other thread blocks' shares: only once it is asked for) */
+/* What the ring holds before the first tile: the choice's own tables, then, as long as the launch needs them, the scores of a chunk
+ * of blocks behind the best of the chunks before. */
+struct ChoiceTables {
+    double qsum[256];
     float list_score[SP_LIST], best[SP_THREADS];
     uint32_t list[SP_LIST];
-    uint32_t ids[SILVANN_B200_PAGED_KEEP_MAX], picked[SILVANN_B200_PAGED_KEEP_MAX];
-    double qsum[256];
     uint32_t warp_in[SP_WARPS], warp_tie[SP_WARPS];
-    uint32_t bin, need;
-    __device__ __forceinline__ uint32_t* hist() { return (uint32_t*)best; }          /* [256], where the floats did not tell */
-    __device__ __forceinline__ unsigned long long key(uint32_t i) const { return (unsigned long long)key_hi[i] << 32 | key_lo[i]; }
+    uint32_t bin, need, pad;
+    float least;
+};
+struct Choice {
+    ChoiceTables* t;
+    uint32_t cap, top;                                                                            /* multiples of four */
+    __device__ __forceinline__ float* score() const { return (float*)(t + 1); }                   /* [cap] to the nearest float: tells all but the closest apart; NaN where there is none */
+    __device__ __forceinline__ int32_t* place() const { return (int32_t*)score() + cap; }         /* [cap] the block's number in the pool, -1: none */
+    __device__ __forceinline__ uint32_t* key_hi() const { return (uint32_t*)score() + 2u * cap; } /* [cap] the score's 64-bit key (of the cluster's other thread blocks' */
+    __device__ __forceinline__ uint32_t* key_lo() const { return (uint32_t*)score() + 3u * cap; } /* [cap] shares: only once it is asked for) */
+    __device__ __forceinline__ uint32_t* ids() const { return (uint32_t*)score() + 4u * cap; }    /* [top] */
+    __device__ __forceinline__ uint32_t* picked() const { return ids() + top; }                   /* [top] */
+    __device__ __forceinline__ uint32_t* hist() const { return (uint32_t*)t->best; }              /* [256], where the floats did not tell */
+    __device__ __forceinline__ unsigned long long key(uint32_t i) const { return (unsigned long long)key_hi()[i] << 32 | key_lo()[i]; }
 };
 
 /* A histogram walked down from its top bin by one warp: the bin where the count reaches `need`, and what is still needed in it. */
-__device__ __forceinline__ void hist_walk(ChoiceSmem& S, uint32_t need, int lane) {
+__device__ __forceinline__ void hist_walk(const Choice S, uint32_t need, int lane) {
     uint32_t mine = 0u;
     for (int b = 0; b < 8; ++b) mine += S.hist()[255 - 8 * lane - b];
     uint32_t upto = mine;
@@ -127,13 +136,13 @@ __device__ __forceinline__ void hist_walk(ChoiceSmem& S, uint32_t need, int lane
     if (lane == __ffs(reached) - 1) {
         uint32_t covered = upto - mine, bin = 255u - 8u * (uint32_t)lane;
         for (int b = 0; b < 7 && covered + S.hist()[bin] < need; ++b) covered += S.hist()[bin--];
-        S.bin = bin; S.need = need - covered;
+        S.t->bin = bin; S.t->need = need - covered;
     }
 }
 
 /* Where many scores are equal, or many blocks are chosen: the `take`-th greatest key found a byte at a time, then two passes
  * over all keys, one that counts and one that writes, in index order. */
-__device__ __noinline__ void choose_by_bytes(ChoiceSmem& S, uint32_t m, uint32_t take) {
+__device__ __noinline__ void choose_by_bytes(const Choice S, uint32_t m, uint32_t take) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned long long known = 0ull, cut = 0ull;
     uint32_t ties = take;
@@ -145,7 +154,7 @@ __device__ __noinline__ void choose_by_bytes(ChoiceSmem& S, uint32_t m, uint32_t
         __syncthreads();
         if (warp == 0) hist_walk(S, ties, lane);
         __syncthreads();
-        cut |= (unsigned long long)S.bin << shift; ties = S.need; known |= 255ull << shift;
+        cut |= (unsigned long long)S.t->bin << shift; ties = S.t->need; known |= 255ull << shift;
         __syncthreads();
     }
     /* every key above the cut and the first `ties` of those that equal it; each warp owns a run of indexes */
@@ -154,10 +163,10 @@ __device__ __noinline__ void choose_by_bytes(ChoiceSmem& S, uint32_t m, uint32_t
     for (uint32_t i = i0 + lane; i < i0 + run; i += 32) {
         n_in += __popc(__ballot_sync(0xffffffffu, i < m && S.key(i) > cut)); n_tie += __popc(__ballot_sync(0xffffffffu, i < m && S.key(i) == cut));
     }
-    if (lane == 0) { S.warp_in[warp] = n_in; S.warp_tie[warp] = n_tie; }
+    if (lane == 0) { S.t->warp_in[warp] = n_in; S.t->warp_tie[warp] = n_tie; }
     __syncthreads();
     uint32_t at = 0u, tied = 0u;
-    for (int w = 0; w < warp; ++w) { at += S.warp_in[w]; tied += S.warp_tie[w]; }
+    for (int w = 0; w < warp; ++w) { at += S.t->warp_in[w]; tied += S.t->warp_tie[w]; }
     at += min(tied, ties);
     const unsigned below = (1u << lane) - 1u;
     for (uint32_t i = i0 + lane; i < i0 + run; i += 32) {
@@ -165,15 +174,15 @@ __device__ __noinline__ void choose_by_bytes(ChoiceSmem& S, uint32_t m, uint32_t
         const unsigned tb = __ballot_sync(0xffffffffu, tie);
         const bool in = (i < m && S.key(i) > cut) || (tie && tied + __popc(tb & below) < ties);
         const unsigned ib = __ballot_sync(0xffffffffu, in);
-        if (in) S.picked[at + __popc(ib & below)] = i;
+        if (in) S.picked()[at + __popc(ib & below)] = i;
         at += __popc(ib); tied += __popc(tb);
     }
     __syncthreads();
 }
 
 /* A number that exactly `take` of score[0..n) reach, n <= 32 K, or NaN when there is none: equal floats lie across the border,
- * or infinities do.  The interval between the least and the greatest finite score is halved; every warp holds all scores and counts
- * for itself, so that a step is a compare, a vote and a population count, without a barrier. */
+ * or infinities do.  The interval between the least and the greatest finite score is halved by one warp that holds all scores, so that a
+ * step is a compare, a vote and a population count, without a barrier. */
 template <int K>
 __device__ __forceinline__ float border(const float* score, uint32_t n, uint32_t take, float (&w)[K]) {
     const uint32_t lane = threadIdx.x & 31u;
@@ -202,33 +211,37 @@ __device__ __forceinline__ float border(const float* score, uint32_t n, uint32_t
 }
 
 /* The indexes of the `take` greatest of score[0..n) into S.picked, ascending, by that border (index[] of them where there is one);
- * false when there is none.  Each warp writes its share of what all of them hold. */
+ * false when there is none.  One warp's work (all eight doing the same was slower: they share four schedulers). */
 template <int K>
-__device__ __noinline__ bool choose_by_border(ChoiceSmem& S, const float* score, const uint32_t* index, uint32_t n, uint32_t take) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    float w[K];
-    const float least = border<K>(score, n, take, w);
-    if (!(least == least)) return false;
-    uint32_t at = 0u;
+__device__ __noinline__ bool choose_by_border(const Choice S, const float* score, const uint32_t* index, uint32_t n, uint32_t take) {
+    const uint32_t lane = threadIdx.x & 31u;
+    if (threadIdx.x < 32u) {
+        float w[K];
+        const float least = border<K>(score, n, take, w);
+        uint32_t at = 0u;
+        if (least == least) {
 #pragma unroll
-    for (int x = 0; x < K; ++x) {
-        const unsigned in = __ballot_sync(0xffffffffu, w[x] >= least);
-        if (x % SP_WARPS == warp && w[x] >= least) S.picked[at + __popc(in & ((1u << lane) - 1u))] = index ? index[x * 32u + lane] : x * 32u + lane;
-        at += __popc(in);
+            for (int x = 0; x < K; ++x) {
+                const unsigned in = __ballot_sync(0xffffffffu, w[x] >= least);
+                if (w[x] >= least) S.picked()[at + __popc(in & ((1u << lane) - 1u))] = index ? index[x * 32u + lane] : x * 32u + lane;
+                at += __popc(in);
+            }
+        }
+        if (lane == 0u) S.t->need = at;
     }
     __syncthreads();
-    return true;
+    return S.t->need == take;
 }
 
 /* The `take` greatest of the m scores (equal ones: the lower index), their indexes ascending into S.picked; m > take > 0; false when the
  * floats do not tell: the 64-bit keys have to (choose_by_bytes).  Called by SP_THREADS threads, with the same answer in all of them.
  * Up to 512 scores: by their border.  More: first the border among the threads' own greatest — `take` of them reach it, so at least
  * `take` scores do, and, scores being in no order, not many more: they are listed, in order, and chosen from. */
-__device__ __forceinline__ bool choose(ChoiceSmem& S, uint32_t m, uint32_t take) {
+__device__ __forceinline__ bool choose(const Choice S, uint32_t m, uint32_t take) {
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    if (m <= 128u) return choose_by_border<4>(S, S.score, nullptr, m, take);
-    if (m <= 256u) return choose_by_border<8>(S, S.score, nullptr, m, take);
-    if (m <= SP_LIST) return choose_by_border<16>(S, S.score, nullptr, m, take);
+    if (m <= 128u) return choose_by_border<4>(S, S.score(), nullptr, m, take);
+    if (m <= 256u) return choose_by_border<8>(S, S.score(), nullptr, m, take);
+    if (m <= SP_LIST) return choose_by_border<16>(S, S.score(), nullptr, m, take);
     if (take > SP_THREADS) return false;
     /* a thread's scores are neighbours, so that the list is in order */
     constexpr int MOST = (SP_CAP + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u);        /* loads of four */
@@ -236,33 +249,38 @@ __device__ __forceinline__ bool choose(ChoiceSmem& S, uint32_t m, uint32_t take)
     float best = __int_as_float(0x7FFFFFFF);
 #pragma unroll
     for (int x = 0; x < MOST; ++x)
-        if (4u * x < run && i0 + 4u * x < m) { const float4 y = *reinterpret_cast<const float4*>(S.score + i0 + 4 * x); best = fmaxf(best, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w))); }
-    S.best[tid] = best;
+        if (4u * x < run && i0 + 4u * x < m) { const float4 y = *reinterpret_cast<const float4*>(S.score() + i0 + 4 * x); best = fmaxf(best, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w))); }
+    S.t->best[tid] = best;
     __syncthreads();
     float w[SP_THREADS / 32];
-    const float least = border<SP_THREADS / 32>(S.best, SP_THREADS, take, w);
+    if (warp == 0u) {
+        const float found = border<SP_THREADS / 32>(S.t->best, SP_THREADS, take, w);
+        if (lane == 0u) S.t->least = found;
+    }
+    __syncthreads();
+    const float least = S.t->least;
     if (!(least == least)) return false;
     uint32_t hits = 0u;
 #pragma unroll
     for (int x = 0; x < MOST; ++x)
         if (4u * x < run && i0 + 4u * x < m) {
-            const float4 y = *reinterpret_cast<const float4*>(S.score + i0 + 4 * x);
+            const float4 y = *reinterpret_cast<const float4*>(S.score() + i0 + 4 * x);
             hits |= ((y.x >= least ? 1u : 0u) | (y.y >= least ? 2u : 0u) | (y.z >= least ? 4u : 0u) | (y.w >= least ? 8u : 0u)) << (4 * x);
         }
     uint32_t upto = __popc(hits);
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
-    if (lane == 31u) S.warp_in[warp] = upto;
+    if (lane == 31u) S.t->warp_in[warp] = upto;
     __syncthreads();
     uint32_t at = upto - __popc(hits), n = 0u;
 #pragma unroll
-    for (uint32_t x = 0; x < SP_WARPS; ++x) { const uint32_t c = S.warp_in[x]; if (x < warp) at += c; n += c; }
+    for (uint32_t x = 0; x < SP_WARPS; ++x) { const uint32_t c = S.t->warp_in[x]; if (x < warp) at += c; n += c; }
     if (n > SP_LIST) return false;
-    for (; hits; hits &= hits - 1u, ++at) { const uint32_t i = i0 + __ffs(hits) - 1u; S.list[at] = i; S.list_score[at] = S.score[i]; }
+    for (; hits; hits &= hits - 1u, ++at) { const uint32_t i = i0 + __ffs(hits) - 1u; S.t->list[at] = i; S.t->list_score[at] = S.score()[i]; }
     __syncthreads();
-    if (n <= 128u) return choose_by_border<4>(S, S.list_score, S.list, n, take);
-    if (n <= 256u) return choose_by_border<8>(S, S.list_score, S.list, n, take);
-    return choose_by_border<16>(S, S.list_score, S.list, n, take);
+    if (n <= 128u) return choose_by_border<4>(S, S.t->list_score, S.t->list, n, take);
+    if (n <= 256u) return choose_by_border<8>(S, S.t->list_score, S.t->list, n, take);
+    return choose_by_border<16>(S, S.t->list_score, S.t->list, n, take);
 }
 
 /* The score of a mean that holds an infinity or a NaN (any of a warp's `count`): summed by conversion.  Such a score is no finite number
@@ -295,7 +313,7 @@ __device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) 
 }
 
 template <int D, int DT, int NHT>
-__global__ void __launch_bounds__(SP_THREADS, 2)
+__global__ void __launch_bounds__(SP_THREADS, SparseCfg<D>::OCC)
 paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const SparseParams P) {
     using Cfg = SparseCfg<D>;
     using E = Elem<DT>;
@@ -308,8 +326,8 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     uint8_t* smem = (uint8_t*)(((uintptr_t)sp_raw + 1023) & ~(uintptr_t)1023);
     const uint32_t keep = P.first + P.last + P.top;
     uint8_t* ring = smem;
-    ChoiceSmem& S = *(ChoiceSmem*)ring;
-    uint8_t* q_base = ring + Cfg::STAGES * Cfg::STAGE_BYTES;
+    const Choice S = {(ChoiceTables*)ring, P.cap, P.choice_top};
+    uint8_t* q_base = ring + P.ring_bytes;
     float* meet = (float*)(q_base + Q_BYTES);                     /* [CL][HPB][D / CL] partials of this block's columns, from every peer */
     float* meet_ml = meet + HPB * D;                              /* [16][HPB][2] */
     uint64_t* full = (uint64_t*)(meet_ml + 16 * HPB * 2);
@@ -397,7 +415,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     const bool fixed = (uint32_t)tid < c.count && !((uint32_t)tid >= c.lo && (uint32_t)tid < c.lo + c.take);
     const int32_t fixed_at = fixed ? paged_block(row, P.stride, P.pool_pages, P.per, always(tid)) : 0;
     if (c.take) {
-        const uint32_t chunk = min(SP_CHUNK, c.hi - c.lo), per = share(chunk), from = min(chunk, crank * per);
+        const uint32_t chunk = min(P.chunk, c.hi - c.lo), per = share(chunk), from = min(chunk, crank * per);
         mine = look_up(c.lo + from, min(per, chunk - from), 0u);
         load(mine);
     }
@@ -407,7 +425,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         if (h < HPB) *reinterpret_cast<uint4*>(q_base + (j / 8) * (HPB * 128) + swz128(h, j % 8)) = qv[z];
     }
     /* the summed query in pairs, a round's pairs side by side for the lanes that share a mean */
-    if (P.top && tid < D) S.qsum[((((tid / 8) / Cfg::LPB) * 4 + (tid % 8) / 2) * Cfg::LPB + (tid / 8) % Cfg::LPB) * 2 + tid % 2] = qs * W::up();
+    if (P.top && tid < D) S.t->qsum[((((tid / 8) / Cfg::LPB) * 4 + (tid % 8) / 2) * Cfg::LPB + (tid / 8) % Cfg::LPB) * 2 + tid % 2] = qs * W::up();
     for (uint32_t i = tid; i < keep; i += SP_THREADS) {
         if (i >= c.lo && i < c.lo + c.take) continue;
         if (i < c.count) {
@@ -421,10 +439,10 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     if (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     /* ---- scores and choice, a chunk of blocks at a time ---- */
-    const bool many = c.hi - c.lo > SP_CHUNK;
+    const bool many = c.hi - c.lo > P.chunk;
     uint32_t have = 0;                                                    /* the best of the chunks so far: keys, place, ids [0..have) */
-    for (uint32_t base = c.lo; c.take && base < c.hi; base += SP_CHUNK) {
-        const uint32_t chunk = min(SP_CHUNK, c.hi - base), per = share(chunk), from = min(chunk, crank * per), n = min(per, chunk - from);
+    for (uint32_t base = c.lo; c.take && base < c.hi; base += P.chunk) {
+        const uint32_t chunk = min(P.chunk, c.hi - base), per = share(chunk), from = min(chunk, crank * per), n = min(per, chunk - from);
         const uint32_t front = (have + 3u) & ~3u;                         /* where the chunk's scores begin, on sixteen bytes */
         {
             if (base != c.lo) { mine = look_up(base + from, n, 0u); load(mine); }
@@ -441,7 +459,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                         double a[4] = {0, 0, 0, 0};
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            const double2 q2 = *reinterpret_cast<const double2*>(S.qsum + ((y * 4 + z) * Cfg::LPB + lane % Cfg::LPB) * 2);
+                            const double2 q2 = *reinterpret_cast<const double2*>(S.t->qsum + ((y * 4 + z) * Cfg::LPB + lane % Cfg::LPB) * 2);
 #pragma unroll
                             for (int u = g; u < g + 4; ++u) {
                                 const uint32_t w = z == 0 ? x[u][y].x : z == 1 ? x[u][y].y : z == 2 ? x[u][y].z : x[u][y].w;
@@ -470,25 +488,25 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 const int u = (up0 ? 4 : 0) + (up1 ? 2 : 0) + (up2 ? 1 : 0);
                 const int32_t at = __shfl_sync(0xffffffffu, old, u * Cfg::BPS + lane / Cfg::LPB);
                 if (__any_sync(0xffffffffu, (special & 0xFFFFu) >= W::SPECIAL || (special >> 16) >= W::SPECIAL))
-                    v = special_score<D, DT>(P.means + (size_t)kvh * D, P.kv_heads * D, old, Cfg::WB, S.qsum, u * Cfg::BPS + lane / Cfg::LPB, v, Cfg::LPB);
+                    v = special_score<D, DT>(P.means + (size_t)kvh * D, P.kv_heads * D, old, Cfg::WB, S.t->qsum, u * Cfg::BPS + lane / Cfg::LPB, v, Cfg::LPB);
                 const uint32_t i = i0 + u * STRIDE + w_at + lane / Cfg::LPB;
                 if (i < n && lane % T2 == 0) {
                     const double score = at >= 0 ? v : -INFINITY;
                     const unsigned long long k = score_key(score);
                     const uint32_t z = front + from + i;
-                    S.score[z] = score_float<DT>(score); S.key_hi[z] = (uint32_t)(k >> 32); S.key_lo[z] = (uint32_t)k; S.place[z] = at;
+                    S.score()[z] = score_float<DT>(score); S.key_hi()[z] = (uint32_t)(k >> 32); S.key_lo()[z] = (uint32_t)k; S.place()[z] = at;
                 }
             }
         }
         /* between the best of the chunks before and this chunk, and behind it: no scores, and keys that none has */
         if (tid < 4u) {
-            if (have + tid < front) { S.score[have + tid] = __int_as_float(0x7FFFFFFF); S.key_hi[have + tid] = 0u; S.key_lo[have + tid] = 0u; }
-            S.score[front + chunk + tid] = __int_as_float(0x7FFFFFFF); S.key_hi[front + chunk + tid] = 0u; S.key_lo[front + chunk + tid] = 0u;
+            if (have + tid < front) { S.score()[have + tid] = __int_as_float(0x7FFFFFFF); S.key_hi()[have + tid] = 0u; S.key_lo()[have + tid] = 0u; }
+            S.score()[front + chunk + tid] = __int_as_float(0x7FFFFFFF); S.key_hi()[front + chunk + tid] = 0u; S.key_lo()[front + chunk + tid] = 0u;
         }
         /* this thread block's share of two arrays to every peer, four entries at a time (behind the chunk's last there is the same everywhere) */
         auto send = [&](const uint32_t* two) {
             for (uint32_t z = tid >> 1; z < (n + 3u) / 4u; z += SP_THREADS / 2u) {
-                const uint32_t* src = two + (tid & 1u) * SP_CAP + front + from + z * 4u;
+                const uint32_t* src = two + (tid & 1u) * S.cap + front + from + z * 4u;
                 const uint4 y = *reinterpret_cast<const uint4*>(src);
 #pragma unroll 4
                 for (uint32_t to = 0; to < CL; ++to)
@@ -497,19 +515,19 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         };
         __syncthreads();
         if (CL > 1) {
-            send((const uint32_t*)S.score);
-            if (many) send(S.key_hi);                                     /* the best go on to the next chunk with their keys */
+            send((const uint32_t*)S.score());
+            if (many) send(S.key_hi());                                     /* the best go on to the next chunk with their keys */
             cluster_sync_all();
         }
         const uint32_t m = front + chunk;
-        const bool more = base + SP_CHUNK < c.hi;
+        const bool more = base + P.chunk < c.hi;
         /* (a chunk holds more blocks than can be chosen, or all there are: m > take) */
         if (!choose(S, m, c.take)) {                                      /* all of the cluster's thread blocks come by here, or none */
             __syncthreads();
-            if (CL > 1 && !many) { send(S.key_hi); cluster_sync_all(); }
+            if (CL > 1 && !many) { send(S.key_hi()); cluster_sync_all(); }
             choose_by_bytes(S, m, c.take);
         }
-        auto id_of = [&](uint32_t i) { return i < have ? S.ids[i] : base + (i - front); };
+        auto id_of = [&](uint32_t i) { return i < have ? S.ids()[i] : base + (i - front); };
         if (more) {
             /* the chosen move to the front, in order: read all, then write */
             constexpr int KP = SILVANN_B200_PAGED_KEEP_MAX / SP_THREADS;
@@ -519,21 +537,21 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
             for (int z = 0; z < KP; ++z) {
                 const uint32_t i = tid + z * SP_THREADS;
-                if (i < c.take) { const uint32_t at = S.picked[i]; ks[z] = S.score[at]; kh[z] = S.key_hi[at]; kl[z] = S.key_lo[at]; ii[z] = id_of(at); pp[z] = S.place[at]; }
+                if (i < c.take) { const uint32_t at = S.picked()[i]; ks[z] = S.score()[at]; kh[z] = S.key_hi()[at]; kl[z] = S.key_lo()[at]; ii[z] = id_of(at); pp[z] = S.place()[at]; }
             }
             __syncthreads();
 #pragma unroll
             for (int z = 0; z < KP; ++z) {
                 const uint32_t i = tid + z * SP_THREADS;
-                if (i < c.take) { S.score[i] = ks[z]; S.key_hi[i] = kh[z]; S.key_lo[i] = kl[z]; S.ids[i] = ii[z]; S.place[i] = pp[z]; }
+                if (i < c.take) { S.score()[i] = ks[z]; S.key_hi()[i] = kh[z]; S.key_lo()[i] = kl[z]; S.ids()[i] = ii[z]; S.place()[i] = pp[z]; }
             }
             have = c.take;
             /* no one writes the next scores over what a peer still reads */
             if (CL > 1) cluster_sync_all(); else __syncthreads();
         } else {
             for (uint32_t i = tid; i < c.take; i += SP_THREADS) {
-                const uint32_t at = S.picked[i];
-                slots[c.lo + i] = slot_of(S.place[at]);
+                const uint32_t at = S.picked()[i];
+                slots[c.lo + i] = slot_of(S.place()[at]);
                 if (chosen) chosen[c.lo + i] = (int32_t)id_of(at);
             }
         }
@@ -791,19 +809,27 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 }
 
 template <int D, int DT, int NHT>
-static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& vm, const SparseParams& P, uint64_t units, uint32_t cluster, cudaStream_t st) {
+static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& vm, SparseParams& P, uint64_t units, cudaStream_t st) {
     using Cfg = SparseCfg<D>;
     const uint32_t keep = P.first + P.last + P.top;
-    constexpr size_t fixed = 1024 + (size_t)Cfg::STAGES * Cfg::STAGE_BYTES + Cfg::BOXES * 8 * NHT * 128 + 8 * NHT * (D + 32) * 4 + (2 * Cfg::STAGES + 1) * 8;
-    const size_t smem = fixed + (size_t)keep * 4;
-    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= sizeof(ChoiceSmem), "the scores fit the ring");
-    static_assert(offsetof(ChoiceSmem, place) == SP_CAP * 4 && offsetof(ChoiceSmem, key_lo) == offsetof(ChoiceSmem, key_hi) + SP_CAP * 4, "arrays that are sent lie in pairs");
-    static_assert(fixed + SILVANN_B200_PAGED_KEEP_MAX * 4 <= 227 * 1024, "a thread block's shared memory");
-    static_assert((size_t)Cfg::STAGES * Cfg::STAGE_BYTES >= (size_t)Cfg::PW * 8 * NHT * (D + 6) * 4, "the partials fit the ring");
+    constexpr size_t rest = 1024 + Cfg::BOXES * 8 * NHT * 128 + 8 * NHT * (D + 32) * 4 + (2 * Cfg::STAGES + 1) * 8;
+    constexpr size_t ring = (size_t)Cfg::STAGES * Cfg::STAGE_BYTES, choice_most = sizeof(ChoiceTables) + 16 * (SP_CAP + 4) + 8 * SILVANN_B200_PAGED_KEEP_MAX;
+    static_assert(rest + (ring > choice_most ? ring : choice_most) + 127 + SILVANN_B200_PAGED_KEEP_MAX * 4 <= 227 * 1024, "a thread block's shared memory");
+    static_assert(ring >= (size_t)Cfg::PW * 8 * NHT * (D + 6) * 4, "the partials fit the ring");
+    static_assert(sizeof(ChoiceTables) % 16 == 0, "the scores begin on sixteen bytes");
+    const size_t choice = sizeof(ChoiceTables) + 16 * (size_t)P.cap + 8 * (size_t)P.choice_top;
+    P.ring_bytes = (uint32_t)((P.top && choice > ring ? choice : ring) + 127) & ~127u;
+    const size_t smem = rest + P.ring_bytes + (size_t)keep * 4;
+    constexpr size_t most = rest + (ring > choice_most ? ring : choice_most) + 127 + SILVANN_B200_PAGED_KEEP_MAX * 4;
+    /* As many thread blocks a row as fit the card at once, as far as a row's longest list of tiles goes round. */
+    const uint32_t fit = (uint32_t)(228 * 1024 / (smem + 1024)), slots = device_sm_count() * (fit < (uint32_t)Cfg::OCC ? fit : (uint32_t)Cfg::OCC);
+    const uint32_t tiles = (keep * P.block + Cfg::TP - 1u) / Cfg::TP;
+    uint32_t cluster = 1u;
+    while (cluster < 16u && units * cluster * 2u <= slots && cluster < tiles) cluster *= 2u;
     static std::atomic<bool> attr_set[SPARSE_DEVICES];
     int d = 0; cudaGetDevice(&d);
     if (d >= 0 && d < SPARSE_DEVICES && !attr_set[d].load(std::memory_order_acquire)) {
-        cudaError_t e = cudaFuncSetAttribute(paged_sparse_kernel<D, DT, NHT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + SILVANN_B200_PAGED_KEEP_MAX * 4));
+        cudaError_t e = cudaFuncSetAttribute(paged_sparse_kernel<D, DT, NHT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_sparse_kernel<D, DT, NHT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         attr_set[d].store(true, std::memory_order_release);
@@ -817,7 +843,7 @@ static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& v
         if (cluster > 1u) { at[na].id = cudaLaunchAttributeClusterDimension; at[na].val.clusterDim.x = cluster; at[na].val.clusterDim.y = 1; at[na].val.clusterDim.z = 1; ++na; }
         if (pdl_allowed()) { at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[na].val.programmaticStreamSerializationAllowed = 1; ++na; }
         cfg.attrs = at; cfg.numAttrs = na;
-        e = cudaLaunchKernelEx(&cfg, paged_sparse_kernel<D, DT, NHT>, km, vm, P);
+        e = cudaLaunchKernelEx(&cfg, paged_sparse_kernel<D, DT, NHT>, km, vm, (const SparseParams)P);
         if (e == cudaSuccess) { note_launch(1); return cudaGetLastError(); }
         (void)cudaGetLastError();
     }
@@ -828,16 +854,20 @@ static cudaError_t sparse_launch(SparseParams& P, const void* k, const void* v, 
     const uint32_t nht = P.group <= 8u ? 1u : 2u;
     P.head_blocks = (P.group + 8u * nht - 1u) / (8u * nht);
     const uint64_t units = (uint64_t)rows * P.kv_heads * P.head_blocks, cols = (uint64_t)P.kv_heads * d;
-    /* As many thread blocks a row as fit the card at once, two an SM, as far as a row's longest list of tiles goes round. */
-    const uint32_t sms = device_sm_count() * 2u, tp = d == 256 ? 32u : 64u, tiles = ((P.first + P.last + P.top) * P.block + tp - 1u) / tp;
-    uint32_t cluster = 1u;
-    while (cluster < 16u && units * cluster * 2u <= sms && cluster < tiles) cluster *= 2u;
+    const uint32_t tp = d == 256 ? 32u : d == 128 ? 64u : 128u;
+    /* a chunk holds all the blocks a table row can name, or more than can be chosen */
+    const uint64_t most = (uint64_t)P.stride * P.per.d;
+    P.choice_top = (P.top + 3u) & ~3u;
+    P.chunk = (uint32_t)(most < SP_CHUNK ? most : SP_CHUNK);
+    if (P.chunk < P.top + 4u) P.chunk = P.top + 4u;
+    P.chunk = (P.chunk + 3u) & ~3u;
+    P.cap = P.chunk + P.choice_top + 8u;
     CUtensorMap km, vm;
     const bool bf = dtype == SV_DTYPE_BF16;
     const uint32_t box = P.block < tp ? P.block : tp;
     if (!make_map_2d_sw128(&km, k, cols, (uint64_t)P.pool_pages * P.page_pos, cols * 2u, 64u, box, bf) || !make_map_2d_sw128(&vm, v, cols, (uint64_t)P.pool_pages * P.page_pos, cols * 2u, 64u, box, bf))
         return cudaErrorInvalidValue;
-#define SV_SPARSE_CASE(DD, TT) return nht == 1u ? sparse_launch_one<DD, TT, 1>(km, vm, P, units, cluster, st) : sparse_launch_one<DD, TT, 2>(km, vm, P, units, cluster, st)
+#define SV_SPARSE_CASE(DD, TT) return nht == 1u ? sparse_launch_one<DD, TT, 1>(km, vm, P, units, st) : sparse_launch_one<DD, TT, 2>(km, vm, P, units, st)
     if (!bf) { if (d == 64) SV_SPARSE_CASE(64, SV_DTYPE_FP16); else if (d == 128) SV_SPARSE_CASE(128, SV_DTYPE_FP16); else SV_SPARSE_CASE(256, SV_DTYPE_FP16); }
     else { if (d == 64) SV_SPARSE_CASE(64, SV_DTYPE_BF16); else if (d == 128) SV_SPARSE_CASE(128, SV_DTYPE_BF16); else SV_SPARSE_CASE(256, SV_DTYPE_BF16); }
 #undef SV_SPARSE_CASE
