@@ -68,7 +68,7 @@ struct SparseParams {
     uint64_t q_stride;
     PagedDiv per;                       /* blocks a page */
     uint32_t seqs, stride, pool_pages, page_pos, block, q_heads, kv_heads, group, head_blocks, first, last, top;
-    uint32_t chunk, cap, choice_top, ring_bytes;      /* scores looked at in one go, and room for them; the ring, or what lies in its place before */
+    uint32_t table_blocks, chunk, cap, choice_top, ring_bytes;      /* scores looked at in one go, and room for them; the ring, or what lies in its place before */
     float scale_log2;
     bool o_wide;                        /* o starts on 8 bytes */
 };
@@ -378,6 +378,9 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         return;
     }
     const PagedChoice c = paged_choice((uint32_t)pos, P.block, P.first, P.last, P.top);
+    /* blocks that the table row has no column for score minus infinity: of a position far past it, no more of them are looked at than
+     * could be chosen */
+    const uint32_t c_hi = min(c.hi, max(P.table_blocks, c.lo + c.take + 1u));
     const int32_t* row = P.table + (size_t)seq * P.stride;
     bool bad = false;
     /* a block whose page is none is asked for past the pool's last row, where TMA answers zeros */
@@ -415,7 +418,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     const bool fixed = (uint32_t)tid < c.count && !((uint32_t)tid >= c.lo && (uint32_t)tid < c.lo + c.take);
     const int32_t fixed_at = fixed ? paged_block(row, P.stride, P.pool_pages, P.per, always(tid)) : 0;
     if (c.take) {
-        const uint32_t chunk = min(P.chunk, c.hi - c.lo), per = share(chunk), from = min(chunk, crank * per);
+        const uint32_t chunk = min(P.chunk, c_hi - c.lo), per = share(chunk), from = min(chunk, crank * per);
         mine = look_up(c.lo + from, min(per, chunk - from), 0u);
         load(mine);
     }
@@ -439,10 +442,10 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     if (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     /* ---- scores and choice, a chunk of blocks at a time ---- */
-    const bool many = c.hi - c.lo > P.chunk;
+    const bool many = c_hi - c.lo > P.chunk;
     uint32_t have = 0;                                                    /* the best of the chunks so far: keys, place, ids [0..have) */
-    for (uint32_t base = c.lo; c.take && base < c.hi; base += P.chunk) {
-        const uint32_t chunk = min(P.chunk, c.hi - base), per = share(chunk), from = min(chunk, crank * per), n = min(per, chunk - from);
+    for (uint32_t base = c.lo; c.take && base < c_hi; base += P.chunk) {
+        const uint32_t chunk = min(P.chunk, c_hi - base), per = share(chunk), from = min(chunk, crank * per), n = min(per, chunk - from);
         const uint32_t front = (have + 3u) & ~3u;                         /* where the chunk's scores begin, on sixteen bytes */
         {
             if (base != c.lo) { mine = look_up(base + from, n, 0u); load(mine); }
@@ -520,7 +523,7 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             cluster_sync_all();
         }
         const uint32_t m = front + chunk;
-        const bool more = base + P.chunk < c.hi;
+        const bool more = base + P.chunk < c_hi;
         /* (a chunk holds more blocks than can be chosen, or all there are: m > take) */
         if (!choose(S, m, c.take)) {                                      /* all of the cluster's thread blocks come by here, or none */
             __syncthreads();
@@ -858,6 +861,7 @@ static cudaError_t sparse_launch(SparseParams& P, const void* k, const void* v, 
     /* a chunk holds all the blocks a table row can name, or more than can be chosen */
     const uint64_t most = (uint64_t)P.stride * P.per.d;
     P.choice_top = (P.top + 3u) & ~3u;
+    P.table_blocks = (uint32_t)(most < 0x7FFFFFFFull ? most : 0x7FFFFFFFull);
     P.chunk = (uint32_t)(most < SP_CHUNK ? most : SP_CHUNK);
     if (P.chunk < P.top + 4u) P.chunk = P.top + 4u;
     P.chunk = (P.chunk + 3u) & ~3u;

@@ -166,7 +166,7 @@ def bits(rng, shape, dtype, scale=1.0):
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
-@pytest.mark.parametrize("kvh,d,page,block,gap", [(2, 256, 256, 64, 0), (4, 128, 64, 16, 24), (1, 64, 128, 128, 8), (8, 128, 96, 32, 0), (1, 8, 16, 16, 0), (3, 72, 48, 16, 0), (2, 64, 64, 0, 0)])
+@pytest.mark.parametrize("kvh,d,page,block,gap", [(2, 256, 256, 64, 0), (4, 128, 64, 16, 24), (1, 64, 128, 128, 8), (8, 128, 96, 32, 0), (1, 8, 16, 16, 0), (3, 72, 48, 16, 0), (2, 64, 64, 0, 0), (16, 256, 64, 64, 0)])
 def test_write(cuda, dtype, kvh, d, page, block, gap):
     rng = np.random.default_rng(kvh * d + page)
     lens, counts = np.array([0, 1, 15, 63, 64, 200, 7, 31]), np.array([1, 300, 1, 1, 64, 56, 0, 97])
@@ -261,7 +261,7 @@ class Paged:
 
     def run(self, seq, pos, q_heads, first, last, top, q=None, gap=0, want_o=True, want_res=True, table=None, stream=None, means=True):
         cuda, rows, d = self.cuda, len(seq), self.d
-        wide = bits(self.rng, (rows, q_heads * d + gap), self.dtype) if q is None else q
+        self.last_q = wide = bits(self.rng, (rows, q_heads * d + gap), self.dtype) if q is None else q
         keep = first + last + top
         o = cuda.full((rows, q_heads, d), 0x1234, dtype=cuda.int16, device="cuda") if want_o else None
         res = cuda.full((rows, q_heads, d + 2), 77.0, device="cuda") if want_res else None
@@ -423,6 +423,22 @@ def test_sparse_many_rows_with_many_tiles_each(cuda, d, kvh, block, rows, keep):
     P.check(seq, pos, 8 * kvh, *keep, got)
 
 
+def test_sparse_at_a_position_far_past_the_table(cuda):
+    """The last position there can be, over a row of a few columns: the blocks there are, then the lowest of those there are not."""
+    B = 16
+    P = Paged(cuda, 30, [B * 40, 5], 1, 64, 1, B, B)
+    for top in (7, 60):
+        _, o, _, chosen = P.run([0, 1], [2 ** 31 - 1, 2 ** 31 - 1], 4, 1, 2, top)
+        assert ext.device_status() == ref.BAD_PAGE
+        n, have = 2 ** 31 // B, -(-B * 40 // B)
+        got = chosen[0, 0].tolist()
+        assert got[0] == 0 and got[-2:] == [n - 2, n - 1]
+        q = from_bits(P.last_q, 1).astype(np.float64).reshape(2, 4, 64)[0].sum(0)
+        s = from_bits(P.means, 1).astype(np.float64)[P.table[0, :have], 0] @ q
+        order = sorted(range(1, have), key=lambda b: (-s[b], b)) + list(range(have, have + top))
+        assert got[1:-2] == sorted(order[:top]) and np.isfinite(from_bits(o[0], 1)).all()
+
+
 def test_sparse_without_scores_needs_no_means(cuda):
     P = Paged(cuda, 25, [500, 20], 2, 64, 1, 64, 64)
     got = P.run([0, 1], [499, 19], 4, 2, 2, 0, means=False)
@@ -443,6 +459,46 @@ def test_sparse_repeats_and_runs_on_a_stream_of_its_own(cuda):
     c = P.run([0, 1], [2999, 4999], 16, 1, 2, 13, q=q, table=np.where(P.table >= 0, perm[np.maximum(P.table, 0)], -1).astype(np.int32))
     for x, y in zip(a[1:], c[1:]):
         assert np.array_equal(x, y)
+
+
+def test_sparse_outputs_where_the_caller_wants_them(cuda):
+    """No `chosen`; an output that starts on two bytes; either leaves the same bits, and nothing beside them."""
+    P = Paged(cuda, 32, [900, 333], 2, 128, 0, 64, 32)
+    q, o, _, _ = got = P.run([0, 1], [899, 332], 8, 1, 2, 6)
+    P.check([0, 1], [899, 332], 8, 1, 2, 6, got)
+    hold = [dev(cuda, x) for x in (q.reshape(2, -1), P.k, P.v, P.means, np.array([0, 1], np.int32), np.array([899, 332], np.int32), P.table)]
+    wide = cuda.full((2 * 8 * 128 + 3,), 0x1234, dtype=cuda.int16, device="cuda")
+    ext.paged_sparse(wide.data_ptr() + 2, None, None, hold[0], hold[1], hold[2], hold[3], hold[4], hold[5], 2, hold[6], 2, P.table.shape[1], P.pool, 64, 32, 8, 2, 128, 1, 2, 6)
+    cuda.cuda.synchronize()
+    b = host_bits(wide)
+    assert np.array_equal(b[1:-2], o.reshape(-1)) and (b[[0, -2, -1]] == 0x1234).all() and ext.device_status() == 0
+
+
+def test_two_captured_steps_beside_each_other(cuda):
+    """Graphs of two pools replayed at the same time on two streams: the calls share nothing."""
+    made = []
+    for seed, dtype in ((40, 0), (41, 1)):
+        P = Paged(cuda, seed, [4000, 2500, 777], 2, 64, dtype, 64, 16)
+        seq, pos = [0, 1, 2], [3999, 2499, 776]
+        q, o, res, chosen = got = P.run(seq, pos, 16, 1, 2, 20)
+        P.check(seq, pos, 16, 1, 2, 20, got)
+        hold = [dev(cuda, x) for x in (q.reshape(3, -1), P.k, P.v, P.means, np.array(seq, np.int32), np.array(pos, np.int32), P.table)]
+        out, ids = cuda.zeros((3, 16, 64), dtype=cuda.int16, device="cuda"), i32(cuda, 3, 2, 23)
+        graph, stream = cuda.cuda.CUDAGraph(), cuda.cuda.Stream()
+        with cuda.cuda.graph(graph, stream=stream):
+            for _ in range(20):
+                ext.paged_sparse(out, None, ids, hold[0], hold[1], hold[2], hold[3], hold[4], hold[5], 3, hold[6], 3, P.table.shape[1], P.pool, 64, 16, 16, 2, 64, 1, 2, 20, dtype=dtype,
+                                 stream=cuda.cuda.current_stream().cuda_stream)
+        made.append((graph, stream, out, ids, o, chosen, hold))
+    cuda.cuda.synchronize()
+    for _ in range(5):
+        for graph, stream, *_ in made:
+            with cuda.cuda.stream(stream):
+                graph.replay()
+    cuda.cuda.synchronize()
+    for _, _, out, ids, o, chosen, _ in made:
+        assert np.array_equal(host_bits(out), o) and np.array_equal(ids.cpu().numpy(), chosen)
+    assert ext.device_status() == 0
 
 
 def test_sparse_with_every_block_kept_is_the_paged_decode(cuda):
