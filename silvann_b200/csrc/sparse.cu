@@ -82,15 +82,15 @@ template <> struct Wide<SV_DTYPE_BF16> {
     static constexpr int SHIFT = 96;
     static constexpr uint32_t SPECIAL = 0x7F80u;
     static __device__ __forceinline__ double up() { return __hiloint2double((800 + 1023) << 20, 0); }
-    static __device__ __forceinline__ double lo(uint32_t w) { return __hiloint2double((int)(((w & 0x8000u) << 16) | ((w & 0x7FFFu) << 13)), 0); }
-    static __device__ __forceinline__ double hi(uint32_t w) { return __hiloint2double((int)((w & 0x80000000u) | ((w & 0x7FFF0000u) >> 3)), 0); }
+    static __device__ __forceinline__ double hi(uint32_t w) { return __hiloint2double(((int)w >> 3) & (int)0x8FFFE000, 0); }      /* (the sign stays, its copies go) */
+    static __device__ __forceinline__ double lo(uint32_t w) { return hi(w << 16); }
 };
 template <> struct Wide<SV_DTYPE_FP16> {
     static constexpr int SHIFT = 108;
     static constexpr uint32_t SPECIAL = 0x7C00u;
     static __device__ __forceinline__ double up() { return __hiloint2double((900 + 1023) << 20, 0); }
-    static __device__ __forceinline__ double lo(uint32_t w) { return __hiloint2double((int)(((w & 0x8000u) << 16) | ((w & 0x7FFFu) << 10)), 0); }
-    static __device__ __forceinline__ double hi(uint32_t w) { return __hiloint2double((int)((w & 0x80000000u) | ((w & 0x7FFF0000u) >> 6)), 0); }
+    static __device__ __forceinline__ double hi(uint32_t w) { return __hiloint2double(((int)w >> 6) & (int)0x81FFFC00, 0); }      /* (the sign stays, its copies go) */
+    static __device__ __forceinline__ double lo(uint32_t w) { return hi(w << 16); }
 };
 
 /* Orders as the score does, NaN with minus infinity. */
@@ -403,9 +403,9 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         return at;
     };
     uint4 x[Cfg::U][Cfg::CPL];
-    auto load = [&](int32_t mine) {
+    auto load = [&](int32_t mine, int g) {                /* rounds g to g + 3 */
 #pragma unroll
-        for (int u = 0; u < Cfg::U; ++u) {
+        for (int u = g; u < g + 4; ++u) {
             const int32_t at = __shfl_sync(0xffffffffu, mine, u * Cfg::BPS + lane / Cfg::LPB);
             const uint4* src = reinterpret_cast<const uint4*>(P.means + ((size_t)max(at, 0) * P.kv_heads + kvh) * D) + lane % Cfg::LPB;
 #pragma unroll
@@ -420,7 +420,9 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     if (c.take) {
         const uint32_t chunk = min(P.chunk, c_hi - c.lo), per = share(chunk), from = min(chunk, crank * per);
         mine = look_up(c.lo + from, min(per, chunk - from), 0u);
-        load(mine);
+        next = look_up(c.lo + from, min(per, chunk - from), STRIDE * Cfg::U);
+        load(mine, 0);
+        load(mine, 4);
     }
 #pragma unroll
     for (int z = 0; z < QV; ++z) {
@@ -448,15 +450,17 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         const uint32_t chunk = min(P.chunk, c_hi - base), per = share(chunk), from = min(chunk, crank * per), n = min(per, chunk - from);
         const uint32_t front = (have + 3u) & ~3u;                         /* where the chunk's scores begin, on sixteen bytes */
         {
-            if (base != c.lo) { mine = look_up(base + from, n, 0u); load(mine); }
+            if (base != c.lo) { mine = look_up(base + from, n, 0u); next = look_up(base + from, n, STRIDE * Cfg::U); load(mine, 0); load(mine, 4); }
             for (uint32_t i0 = 0; i0 < n; i0 += STRIDE * Cfg::U) {
-                next = look_up(base + from, n, i0 + STRIDE * Cfg::U);
+                /* the places of the round after next, and, as soon as four of this one are multiplied, the next one's four */
+                const int32_t later = look_up(base + from, n, i0 + 2u * STRIDE * Cfg::U);
+                const bool on = i0 + STRIDE * Cfg::U < n;
                 double s[Cfg::U];
                 uint32_t special = 0u;
 #pragma unroll
                 for (int g = 0; g < Cfg::U; g += 4) {
                     s[g] = s[g + 1] = s[g + 2] = s[g + 3] = 0;
-                    if (i0 + g * STRIDE + w_at >= n) continue;
+                    if (i0 + g * STRIDE + w_at < n)
 #pragma unroll
                     for (int y = 0; y < Cfg::CPL; ++y) {
                         double a[4] = {0, 0, 0, 0};
@@ -473,10 +477,10 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
                         for (int u = 0; u < 4; ++u) s[g + u] += a[u];
                     }
+                    if (on) load(next, g);
                 }
                 const int32_t old = mine;
-                mine = next;
-                if (i0 + STRIDE * Cfg::U < n) load(mine);
+                mine = next; next = later;
                 /* the lanes' parts of eight means at once: each exchange halves what a lane still holds; whichever of two lanes
                  * adds, the sum is the same */
                 constexpr int T0 = Cfg::LPB / 2, T1 = Cfg::LPB / 4, T2 = Cfg::LPB / 8;
