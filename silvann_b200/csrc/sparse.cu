@@ -68,7 +68,7 @@ struct SparseParams {
     uint64_t q_stride;
     PagedDiv per;                       /* blocks a page */
     uint32_t seqs, stride, pool_pages, page_pos, block, q_heads, kv_heads, group, head_blocks, first, last, top;
-    uint32_t table_blocks, chunk, cap, choice_top, ring_bytes;      /* scores looked at in one go, and room for them; the ring, or what lies in its place before */
+    uint32_t block_log, table_blocks, chunk, cap, choice_top, ring_bytes, choice_at, free_stages;      /* scores looked at in one go, and room for them; the ring, or what lies in its place before, at its end */
     float scale_log2;
     bool o_wide;                        /* o starts on 8 bytes */
 };
@@ -200,7 +200,7 @@ __device__ __forceinline__ float border(const float* score, uint32_t n, uint32_t
         return c; };
     uint32_t c = reach(lo);
     if (c <= take) return c == take ? lo : __int_as_float(0x7FFFFFFF);
-    for (int step = 0; step < 64; ++step) {
+    for (int step = 0; step < 64; ++step) {       /* (a guess by the counts at both ends took fewer steps and more time) */
         const float mid = 0.5f * lo + 0.5f * hi;
         if (!(mid > lo && mid < hi)) break;
         c = reach(mid);
@@ -326,14 +326,14 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     uint8_t* smem = (uint8_t*)(((uintptr_t)sp_raw + 1023) & ~(uintptr_t)1023);
     const uint32_t keep = P.first + P.last + P.top;
     uint8_t* ring = smem;
-    const Choice S = {(ChoiceTables*)ring, P.cap, P.choice_top};
+    const Choice S = {(ChoiceTables*)(ring + P.choice_at), P.cap, P.choice_top};
     uint8_t* q_base = ring + P.ring_bytes;
     float* meet = (float*)(q_base + Q_BYTES);                     /* [CL][HPB][D / CL] partials of this block's columns, from every peer */
     float* meet_ml = meet + HPB * D;                              /* [16][HPB][2] */
     uint64_t* full = (uint64_t*)(meet_ml + 16 * HPB * 2);
     uint64_t* empty = full + Cfg::STAGES;
     volatile uint32_t* abort_flag = (volatile uint32_t*)(empty + Cfg::STAGES);
-    int32_t* slots = (int32_t*)(empty + Cfg::STAGES + 1);         /* [keep] the chosen blocks' places in the pool */
+    int32_t* slots = (int32_t*)(empty + Cfg::STAGES + 1);         /* [keep] the blocks' places in the pool: those always attended, then the chosen, then the row's own */
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t CL = cluster_nctarank(), crank = cluster_ctarank();
@@ -430,17 +430,46 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         if (h < HPB) *reinterpret_cast<uint4*>(q_base + (j / 8) * (HPB * 128) + swz128(h, j % 8)) = qv[z];
     }
     /* the summed query in pairs, a round's pairs side by side for the lanes that share a mean */
-    if (P.top && tid < D) S.t->qsum[((((tid / 8) / Cfg::LPB) * 4 + (tid % 8) / 2) * Cfg::LPB + (tid / 8) % Cfg::LPB) * 2 + tid % 2] = qs * W::up();
+    if (c.take && tid < D) S.t->qsum[((((tid / 8) / Cfg::LPB) * 4 + (tid % 8) / 2) * Cfg::LPB + (tid / 8) % Cfg::LPB) * 2 + tid % 2] = qs * W::up();
     for (uint32_t i = tid; i < keep; i += SP_THREADS) {
         if (i >= c.lo && i < c.lo + c.take) continue;
         if (i < c.count) {
             const int32_t at = i == (uint32_t)tid ? fixed_at : paged_block(row, P.stride, P.pool_pages, P.per, always(i));
             bad |= at < 0;
-            slots[i] = slot_of(at);
+            slots[i < c.lo ? i : i + 1u == c.count ? i : i - c.take] = slot_of(at);
         }
         if (chosen) chosen[i] = i < c.count ? (int32_t)always(i) : -1;
     }
+    /* Tile t of the positions to attend, in the order of `slots`, belongs to thread block t % CL. */
+    const uint32_t live = (c.count - 1u) * P.block + ((uint32_t)pos & (P.block - 1u)) + 1u;      /* the row's own block comes last and may end early */
+    const uint32_t tiles = (live + Cfg::TP - 1u) / Cfg::TP;
+    const int nt = tiles > crank ? (int)((tiles - crank + CL - 1) / CL) : 0;
+
+    /* the loads of tile `it`: one box of 64 columns by min(B, TP) positions a lane of one warp */
+    constexpr uint32_t TP_LOG = Cfg::TP == 32 ? 5u : Cfg::TP == 64 ? 6u : 7u;
+    const uint32_t br_log = min(P.block_log, TP_LOG), br = 1u << br_log;
+    const uint64_t pol = l2_policy_evict_first();
+    auto fetch = [&](int it) {
+        const int s = it % Cfg::STAGES;
+        const uint32_t p0 = (crank + it * CL) * Cfg::TP;
+        const uint32_t boxes = min((uint32_t)Cfg::TP >> br_log, (live - p0 + br - 1u) >> br_log);
+        uint8_t* st = ring + s * Cfg::STAGE_BYTES;
+        if (lane == 0) mbar_expect_tx(&full[s], boxes * br * 128u * Cfg::BOXES * 2u);
+        __syncwarp();
+        for (uint32_t i = lane; i < boxes * Cfg::BOXES * 2u; i += 32) {
+            const uint32_t b = i / (Cfg::BOXES * 2u), x = i % (Cfg::BOXES * 2u), col = x % Cfg::BOXES;
+            const uint32_t at = p0 + b * br;
+            const int32_t y = slots[at >> P.block_log] + (int32_t)(at & (P.block - 1u));
+            tma_load_2d_hint(st + (x / Cfg::BOXES) * Cfg::K_BYTES + col * Cfg::BOX_BYTES + b * br * 128u, x < Cfg::BOXES ? (const void*)&kmap : (const void*)&vmap, &full[s],
+                             (int32_t)(kvh * D + col * 64u), y, pol);
+        }
+        __syncwarp();
+    };
+    /* tiles of blocks that are always attended are asked for ahead of the scores, where the choice's tables leave their stage free */
+    const uint32_t known = c.take ? (c.lo + P.last - 1u) * P.block : live;
+    auto early = [&](int it) { return !c.take || (it < (int)P.free_stages && min((crank + it * CL + 1u) * Cfg::TP, live) <= known); };
     __syncthreads();
+    if (warp < Cfg::STAGES && warp < nt && early(warp)) fetch(warp);
     if (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     /* ---- scores and choice, a chunk of blocks at a time ---- */
@@ -558,18 +587,13 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         } else {
             for (uint32_t i = tid; i < c.take; i += SP_THREADS) {
                 const uint32_t at = S.picked()[i];
-                slots[c.lo + i] = slot_of(S.place()[at]);
+                slots[c.lo + P.last - 1u + i] = slot_of(S.place()[at]);
                 if (chosen) chosen[c.lo + i] = (int32_t)id_of(at);
             }
         }
     }
     fence_proxy_async_smem();            /* the scores' accesses to the ring come before the loads into it */
     __syncthreads();
-
-    /* ---- attend: tile t of the chosen positions belongs to thread block t % CL ---- */
-    const uint32_t live = (c.count - 1u) * P.block + (uint32_t)pos % P.block + 1u;      /* the row's own block is the last and may end early */
-    const uint32_t tiles = (live + Cfg::TP - 1u) / Cfg::TP;
-    const int nt = tiles > crank ? (int)((tiles - crank + CL - 1) / CL) : 0;
 
     float m_run[NHT][2], l_run[NHT][2], oacc[NHT][VS][4];
 #pragma unroll
@@ -578,26 +602,8 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
         for (int k = 0; k < VS; ++k) { oacc[n][k][0] = oacc[n][k][1] = oacc[n][k][2] = oacc[n][k][3] = 0.f; }
     }
-    /* the loads of tile `it`: one box of 64 columns by min(B, TP) positions a lane of one warp */
-    const uint32_t br = min(P.block, (uint32_t)Cfg::TP), sub = Cfg::TP / br;
-    const uint64_t pol = l2_policy_evict_first();
-    auto fetch = [&](int it) {
-        const int s = it % Cfg::STAGES;
-        const uint32_t p0 = (crank + it * CL) * Cfg::TP;
-        const uint32_t boxes = min(sub, (live - p0 + br - 1u) / br);
-        uint8_t* st = ring + s * Cfg::STAGE_BYTES;
-        if (lane == 0) mbar_expect_tx(&full[s], boxes * br * 128u * Cfg::BOXES * 2u);
-        __syncwarp();
-        for (uint32_t i = lane; i < boxes * Cfg::BOXES * 2u; i += 32) {
-            const uint32_t b = i / (Cfg::BOXES * 2u), x = i % (Cfg::BOXES * 2u), col = x % Cfg::BOXES;
-            const uint32_t at = p0 + b * br;
-            const int32_t y = slots[at / P.block] + (int32_t)(at % P.block);
-            tma_load_2d_hint(st + (x / Cfg::BOXES) * Cfg::K_BYTES + col * Cfg::BOX_BYTES + b * br * 128u, x < Cfg::BOXES ? (const void*)&kmap : (const void*)&vmap, &full[s],
-                             (int32_t)(kvh * D + col * 64u), y, pol);
-        }
-        __syncwarp();
-    };
-    if (warp < Cfg::STAGES && warp < nt) fetch(warp);
+    /* ---- attend ---- */
+    if (warp < Cfg::STAGES && warp < nt && !early(warp)) fetch(warp);
     {
         const uint32_t q_u32 = smem_u32(q_base);
         auto load_qfrag = [&](int n, int kk, uint32_t& b0, uint32_t& b1) {
@@ -826,6 +832,8 @@ static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& v
     static_assert(sizeof(ChoiceTables) % 16 == 0, "the scores begin on sixteen bytes");
     const size_t choice = sizeof(ChoiceTables) + 16 * (size_t)P.cap + 8 * (size_t)P.choice_top;
     P.ring_bytes = (uint32_t)((P.top && choice > ring ? choice : ring) + 127) & ~127u;
+    P.choice_at = P.top && choice < P.ring_bytes ? (uint32_t)(P.ring_bytes - choice) & ~127u : 0u;
+    P.free_stages = P.choice_at / Cfg::STAGE_BYTES;
     const size_t smem = rest + P.ring_bytes + (size_t)keep * 4;
     constexpr size_t most = rest + (ring > choice_most ? ring : choice_most) + 127 + SILVANN_B200_PAGED_KEEP_MAX * 4;
     /* As many thread blocks a row as fit the card at once, as far as a row's longest list of tiles goes round. */
@@ -865,6 +873,7 @@ static cudaError_t sparse_launch(SparseParams& P, const void* k, const void* v, 
     /* a chunk holds all the blocks a table row can name, or more than can be chosen */
     const uint64_t most = (uint64_t)P.stride * P.per.d;
     P.choice_top = (P.top + 3u) & ~3u;
+    P.block_log = P.block == 16u ? 4u : P.block == 32u ? 5u : P.block == 64u ? 6u : 7u;
     P.table_blocks = (uint32_t)(most < 0x7FFFFFFFull ? most : 0x7FFFFFFFull);
     P.chunk = (uint32_t)(most < SP_CHUNK ? most : SP_CHUNK);
     if (P.chunk < P.top + 4u) P.chunk = P.top + 4u;
