@@ -16,7 +16,18 @@
  *
  * Why 64 bits for the scores: which block is chosen hangs on two scores next to each other, and a choice that went by the
  * order of a sum in fp32 would be one of the launch's shape.  The products of 16-bit values are exact there and the tree
- * over a mean's columns is the same wherever the mean lies. */
+ * over a mean's columns is the same wherever the mean lies.
+ *
+ * What bounds it.  Many rows of moderate length: memory (256 rows of 1,000 to 16,000 positions, 32 heads on 4 of 128, 16 blocks of 128
+ * each: 175 us, 6.0 TB/s of means, keys and values).  Long rows: the phases' own chains of trips to memory and through shared
+ * memory, during which little is in flight (32 rows of 1,024 to 100,000 positions, 16 heads on 2 of 256: 44 us, of which the tiles
+ * are half; 24 us at memory's rate).  One row: that chain alone (8,192 positions 10.5 us, 262,144 positions 19.1 us in a graph).  Heads
+ * of their own over 16-position blocks: the same and the issue of instructions (24 sequences of 5 drafted positions, 8 heads of 64: 64 us;
+ * 0.46 instructions a cycle and scheduler, 23 % of DRAM).
+ * Measured against, on the same cases: the first launch's two passes over the choice with one barrier a count, or with every key ranked
+ * against every other (a 4,096-block choice: 12 to 20 thousand cycles, now 6.7); scores written to the peers one by one (262,144
+ * positions 22 us); 2 x 64 positions a tile at head_dim 256, one thread block an SM (49 us); means four lanes each instead of eight
+ * (46 us); the tiles of the always attended blocks not asked for early (182 us on the 256 rows). */
 #include "../../include/silvann_b200.h"
 #include "common.cuh"
 #include "kernels.h"
