@@ -118,10 +118,10 @@ __device__ __forceinline__ float score_float(double s) { return s == s ? (float)
  * of blocks behind the best of the chunks before. */
 struct ChoiceTables {
     double qsum[256];
-    float list_score[SP_LIST], best[SP_THREADS];
-    uint32_t list[SP_LIST];
+    float list_score[SP_LIST];
+    uint32_t hist[256], n_list, pad[3];
     uint32_t warp_in[SP_WARPS], warp_tie[SP_WARPS];
-    uint32_t bin, need, pad;
+    uint32_t bin, need, in_bin;
     float least;
 };
 struct Choice {
@@ -133,21 +133,20 @@ struct Choice {
     __device__ __forceinline__ uint32_t* key_lo() const { return (uint32_t*)score() + 3u * cap; } /* [cap] shares: only once it is asked for) */
     __device__ __forceinline__ uint32_t* ids() const { return (uint32_t*)score() + 4u * cap; }    /* [top] */
     __device__ __forceinline__ uint32_t* picked() const { return ids() + top; }                   /* [top] */
-    __device__ __forceinline__ uint32_t* hist() const { return (uint32_t*)t->best; }              /* [256], where the floats did not tell */
     __device__ __forceinline__ unsigned long long key(uint32_t i) const { return (unsigned long long)key_hi()[i] << 32 | key_lo()[i]; }
 };
 
 /* A histogram walked down from its top bin by one warp: the bin where the count reaches `need`, and what is still needed in it. */
 __device__ __forceinline__ void hist_walk(const Choice S, uint32_t need, int lane) {
     uint32_t mine = 0u;
-    for (int b = 0; b < 8; ++b) mine += S.hist()[255 - 8 * lane - b];
+    for (int b = 0; b < 8; ++b) mine += S.t->hist[255 - 8 * lane - b];
     uint32_t upto = mine;
     for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
     const unsigned reached = __ballot_sync(0xffffffffu, upto >= need);
     if (lane == __ffs(reached) - 1) {
         uint32_t covered = upto - mine, bin = 255u - 8u * (uint32_t)lane;
-        for (int b = 0; b < 7 && covered + S.hist()[bin] < need; ++b) covered += S.hist()[bin--];
-        S.t->bin = bin; S.t->need = need - covered;
+        for (int b = 0; b < 7 && covered + S.t->hist[bin] < need; ++b) covered += S.t->hist[bin--];
+        S.t->bin = bin; S.t->need = need - covered; S.t->in_bin = S.t->hist[bin];
     }
 }
 
@@ -158,10 +157,10 @@ __device__ __noinline__ void choose_by_bytes(const Choice S, uint32_t m, uint32_
     unsigned long long known = 0ull, cut = 0ull;
     uint32_t ties = take;
     for (int shift = 56; shift >= 0; shift -= 8) {
-        S.hist()[tid] = 0u;
+        S.t->hist[tid] = 0u;
         __syncthreads();
         for (uint32_t i = tid; i < m; i += SP_THREADS)
-            if ((S.key(i) & known) == cut) atomicAdd(&S.hist()[(uint32_t)(S.key(i) >> shift) & 255u], 1u);
+            if ((S.key(i) & known) == cut) atomicAdd(&S.t->hist[(uint32_t)(S.key(i) >> shift) & 255u], 1u);
         __syncthreads();
         if (warp == 0) hist_walk(S, ties, lane);
         __syncthreads();
@@ -195,8 +194,9 @@ __device__ __noinline__ void choose_by_bytes(const Choice S, uint32_t m, uint32_
  * or infinities do.  The interval between the least and the greatest finite score is halved by one warp that holds all scores, so that a
  * step is a compare, a vote and a population count, without a barrier. */
 template <int K>
-__device__ __forceinline__ float border(const float* score, uint32_t n, uint32_t take, float (&w)[K]) {
+__device__ __forceinline__ float border(const float* score, uint32_t n, uint32_t take) {
     const uint32_t lane = threadIdx.x & 31u;
+    float w[K];
     float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
     for (int x = 0; x < K; ++x) {
@@ -221,78 +221,103 @@ __device__ __forceinline__ float border(const float* score, uint32_t n, uint32_t
     return __int_as_float(0x7FFFFFFF);
 }
 
-/* The indexes of the `take` greatest of score[0..n) into S.picked, ascending, by that border (index[] of them where there is one);
- * false when there is none.  One warp's work (all eight doing the same was slower: they share four schedulers). */
-template <int K>
-__device__ __noinline__ bool choose_by_border(const Choice S, const float* score, const uint32_t* index, uint32_t n, uint32_t take) {
+/* The choice among few scores, one warp's work, four a lane. */
+__device__ __noinline__ bool choose_few(const Choice S, uint32_t m, uint32_t take) {
     const uint32_t lane = threadIdx.x & 31u;
     if (threadIdx.x < 32u) {
-        float w[K];
-        const float least = border<K>(score, n, take, w);
+        const float least = border<4>(S.score(), m, take);
         uint32_t at = 0u;
-        if (least == least) {
+        if (least == least)
 #pragma unroll
-            for (int x = 0; x < K; ++x) {
-                const unsigned in = __ballot_sync(0xffffffffu, w[x] >= least);
-                if (w[x] >= least) S.picked()[at + __popc(in & ((1u << lane) - 1u))] = index ? index[x * 32u + lane] : x * 32u + lane;
+            for (uint32_t i = lane; i < 128u; i += 32u) {
+                const bool is = i < m && S.score()[i] >= least;
+                const unsigned in = __ballot_sync(0xffffffffu, is);
+                if (is) S.picked()[at + __popc(in & ((1u << lane) - 1u))] = i;
                 at += __popc(in);
             }
-        }
         if (lane == 0u) S.t->need = at;
     }
     __syncthreads();
     return S.t->need == take;
 }
 
-/* The `take` greatest of the m scores (equal ones: the lower index), their indexes ascending into S.picked; m > take > 0; false when the
- * floats do not tell: the 64-bit keys have to (choose_by_bytes).  Called by SP_THREADS threads, with the same answer in all of them.
- * Up to 512 scores: by their border.  More: first the border among the threads' own greatest — `take` of them reach it, so at least
- * `take` scores do, and, scores being in no order, not many more: they are listed, in order, and chosen from. */
-__device__ __forceinline__ bool choose(const Choice S, uint32_t m, uint32_t take) {
+/* The choice among many: a histogram of 256 steps of equal width between the least and the greatest finite score finds the step that the
+ * border lies in, which rarely holds more than a few (a tail of scores is thin); one warp finds the border among those. */
+__device__ __noinline__ bool choose_many(const Choice S, uint32_t m, uint32_t take) {
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    if (m <= 128u) return choose_by_border<4>(S, S.score(), nullptr, m, take);
-    if (m <= 256u) return choose_by_border<8>(S, S.score(), nullptr, m, take);
-    if (m <= SP_LIST) return choose_by_border<16>(S, S.score(), nullptr, m, take);
-    if (take > SP_THREADS) return false;
-    /* a thread's scores are neighbours, so that the list is in order */
-    constexpr int MOST = (SP_CAP + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u);        /* loads of four */
-    const uint32_t run = (m + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u) * 4u, i0 = tid * run;
-    float best = __int_as_float(0x7FFFFFFF);
+    /* a thread's scores are neighbours, so that its chosen ones are in order */
+    const uint32_t run = (m + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u) * 4u, i0 = tid * run, i1 = min(m, i0 + run);
+    float mn = INFINITY, mx = -INFINITY;
+    for (uint32_t i = i0; i < i1; i += 4u) {                              /* (behind the last there are NaNs up to a multiple of four) */
+        const float4 y = *reinterpret_cast<const float4*>(S.score() + i);
+        const float f[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int x = 0; x < MOST; ++x)
-        if (4u * x < run && i0 + 4u * x < m) { const float4 y = *reinterpret_cast<const float4*>(S.score() + i0 + 4 * x); best = fmaxf(best, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w))); }
-    S.t->best[tid] = best;
+        for (int x = 0; x < 4; ++x) if (fabsf(f[x]) < INFINITY) { mn = fminf(mn, f[x]); mx = fmaxf(mx, f[x]); }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) { mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, x)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x)); }
+    if (lane == 0u) { S.t->warp_in[warp] = __float_as_uint(mn); S.t->warp_tie[warp] = __float_as_uint(mx); }
+    S.t->hist[tid] = 0u;
+    if (tid == 0u) S.t->n_list = 0u;
     __syncthreads();
-    float w[SP_THREADS / 32];
-    if (warp == 0u) {
-        const float found = border<SP_THREADS / 32>(S.t->best, SP_THREADS, take, w);
-        if (lane == 0u) S.t->least = found;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; ++w) { mn = fminf(mn, __uint_as_float(S.t->warp_in[w])); mx = fmaxf(mx, __uint_as_float(S.t->warp_tie[w])); }
+    const float per = mx > mn ? __fdividef(255.99f, mx - mn) : 0.f, low = mx >= mn ? mn : 0.f;
+    auto bin_of = [&](float f) { return (uint32_t)min(max((int)((f - low) * per), 0), 255); };     /* does not fall as f rises */
+    for (uint32_t i = i0; i < i1; i += 4u) {
+        const float4 y = *reinterpret_cast<const float4*>(S.score() + i);
+        const float f[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) if (f[x] == f[x]) atomicAdd(&S.t->hist[bin_of(f[x])], 1u);
     }
     __syncthreads();
-    const float least = S.t->least;
-    if (!(least == least)) return false;
-    uint32_t hits = 0u;
+    if (warp == 0u) hist_walk(S, take, lane);
+    __syncthreads();
+    const uint32_t bin = S.t->bin, need = S.t->need, in_bin = S.t->in_bin;
+    if (in_bin > SP_LIST) return false;
+    float least = -INFINITY;                      /* of the border's step, what reaches this is chosen */
+    if (in_bin != need) {
+        for (uint32_t i = i0; i < i1; i += 4u) {
+            const float4 y = *reinterpret_cast<const float4*>(S.score() + i);
+            const float f[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int x = 0; x < MOST; ++x)
-        if (4u * x < run && i0 + 4u * x < m) {
-            const float4 y = *reinterpret_cast<const float4*>(S.score() + i0 + 4 * x);
-            hits |= ((y.x >= least ? 1u : 0u) | (y.y >= least ? 2u : 0u) | (y.z >= least ? 4u : 0u) | (y.w >= least ? 8u : 0u)) << (4 * x);
+            for (int x = 0; x < 4; ++x) if (f[x] == f[x] && bin_of(f[x]) == bin) S.t->list_score[atomicAdd(&S.t->n_list, 1u)] = f[x];
         }
+        __syncthreads();
+        if (warp == 0u) {
+            const float found = in_bin <= 32u ? border<1>(S.t->list_score, in_bin, need) : in_bin <= 128u ? border<4>(S.t->list_score, in_bin, need) : border<16>(S.t->list_score, in_bin, need);
+            if (lane == 0u) S.t->least = found;
+        }
+        __syncthreads();
+        least = S.t->least;
+        if (!(least == least)) return false;
+    }
+    uint32_t hits = 0u;
+    for (uint32_t i = i0, b = 0u; i < i1; i += 4u, b += 4u) {
+        const float4 y = *reinterpret_cast<const float4*>(S.score() + i);
+        const float f[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) { const uint32_t z = bin_of(f[x]); hits |= (f[x] == f[x] && (z > bin || (z == bin && f[x] >= least)) ? 1u : 0u) << (b + x); }
+    }
     uint32_t upto = __popc(hits);
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
+    __syncthreads();
     if (lane == 31u) S.t->warp_in[warp] = upto;
     __syncthreads();
-    uint32_t at = upto - __popc(hits), n = 0u;
+    uint32_t at = upto - __popc(hits);
 #pragma unroll
-    for (uint32_t x = 0; x < SP_WARPS; ++x) { const uint32_t c = S.t->warp_in[x]; if (x < warp) at += c; n += c; }
-    if (n > SP_LIST) return false;
-    for (; hits; hits &= hits - 1u, ++at) { const uint32_t i = i0 + __ffs(hits) - 1u; S.t->list[at] = i; S.t->list_score[at] = S.score()[i]; }
+    for (uint32_t x = 0; x < SP_WARPS; ++x) if (x < warp) at += S.t->warp_in[x];
+    for (; hits; hits &= hits - 1u, ++at) S.picked()[at] = i0 + __ffs(hits) - 1u;
     __syncthreads();
-    if (n <= 128u) return choose_by_border<4>(S, S.t->list_score, S.t->list, n, take);
-    if (n <= 256u) return choose_by_border<8>(S, S.t->list_score, S.t->list, n, take);
-    return choose_by_border<16>(S, S.t->list_score, S.t->list, n, take);
+    return true;
 }
+
+/* The `take` greatest of the m scores (equal ones: the lower index), their indexes ascending into S.picked; m > take > 0; false when the
+ * floats do not tell: the 64-bit keys have to (choose_by_bytes).  Called by SP_THREADS threads, with the same answer in all of them.
+ * (125 scores: 2.3 thousand cycles the first way, 3.8 the second, with its barriers; 600 to 1,300: 5 the second way, 7 to 13 by a
+ * warp that holds all of them.) */
+__device__ __forceinline__ bool choose(const Choice S, uint32_t m, uint32_t take) { return m <= 128u ? choose_few(S, m, take) : choose_many(S, m, take); }
 
 /* The score of a mean that holds an infinity or a NaN (any of a warp's `count`): summed by conversion.  Such a score is no finite number
  * whatever the order, so the order is the warp's own.  Answers the score of mean `want`, or `v` where that is an ordinary one. */

@@ -32,9 +32,7 @@ class B200Error(RuntimeError):
 
 
 def addr(x) -> int | None:
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or x.__class__ is int or isinstance(x, int):
         return x
     return x.data_ptr()
 
