@@ -436,7 +436,8 @@ int silvann_b200_paged_write(void* k_pool, void* v_pool, void* k_means, const vo
  * negative is padding: its outputs stay as they were; one with row_seq >= seqs is treated the same and raises
  * SILVANN_B200_STATUS_BAD_PAGE.  A row at a negative position attends nothing: o is 0, res (-inf, 0, 0), chosen -1.
  * head_dim 64, 128 or 256; up to 64 query heads a kv head; B 16, 32, 64 or 128 and a divisor of page_positions;
- * first + last + top <= SILVANN_B200_PAGED_KEEP_MAX; rows of q multiples of 8 elements, addresses of 16 bytes. */
+ * first + last + top <= SILVANN_B200_PAGED_KEEP_MAX; rows * kv_heads <= 2^24; rows of q multiples of 8 elements, addresses of q,
+ * pools and means of 16 bytes. */
 #define SILVANN_B200_PAGED_KEEP_MAX 1024u
 int silvann_b200_paged_sparse(void* o, float* res, int32_t* chosen, const void* q, uint64_t q_stride, const void* k_pool, const void* v_pool,
                               const void* k_means, const int32_t* row_seq, const int32_t* row_pos, uint32_t rows, const int32_t* page_table,

@@ -5,11 +5,11 @@
  * clusters, which make the same choice).  Three phases:
  *
  *   scores  — every block's mean key is read once, from L2 or memory, and multiplied with the sum of the kv head's query
- *             heads; the cluster's thread blocks share the sequence's blocks and leave every score, in 64 bits, in every
- *             thread block's shared memory.
- *   choice  — each thread block picks the same `top` blocks from the whole list, so nothing has to be sent round again.
- *   attend  — the chosen blocks, in order, are a short cache of their own: 64-position tiles of it are dealt to the thread
- *             blocks, arrive by TMA (128-byte swizzle) in a ring, and meet an online softmax with heads as the N dimension
+ *             heads in 64 bits; the cluster's thread blocks share the sequence's blocks and leave every score, as a float, in
+ *             every thread block's shared memory.
+ *   choice  — each thread block picks the same `top` blocks from the whole list, so nothing has to be sent round again: by the
+ *             floats where their order tells, else by the 64 bits, which then follow.
+ *   attend  — the blocks to attend are a short cache of their own: tiles of 32 KB of it are dealt to the thread blocks, arrive by TMA (128-byte swizzle) in a ring, and meet an online softmax with heads as the N dimension
  *             of the warp MMAs (S^T = K Q^T, O^T = V^T P^T).  Some warps share a tile by positions, and their sets share it by value
  *             columns (each set forms the scores, which is cheaper than more accumulators).  The partials
  *             meet through the cluster's shared memory, in a fixed order.  No scratch in global memory: calls share nothing.
@@ -19,15 +19,14 @@
  * over a mean's columns is the same wherever the mean lies.
  *
  * What bounds it.  Many rows of moderate length: memory (256 rows of 1,000 to 16,000 positions, 32 heads on 4 of 128, 16 blocks of 128
- * each: 175 us, 6.0 TB/s of means, keys and values).  Long rows: the phases' own chains of trips to memory and through shared
+ * each: 172 us, 6.1 TB/s of means, keys and values).  Long rows: the phases' own chains of trips to memory and through shared
  * memory, during which little is in flight (32 rows of 1,024 to 100,000 positions, 16 heads on 2 of 256: 44 us, of which the tiles
- * are half; 24 us at memory's rate).  One row: that chain alone (8,192 positions 10.5 us, 262,144 positions 19.1 us in a graph).  Heads
- * of their own over 16-position blocks: the same and the issue of instructions (24 sequences of 5 drafted positions, 8 heads of 64: 64 us;
+ * are half; 24 us at memory's rate).  One row: that chain alone (8,192 positions 10.4 us, 262,144 positions 19.1 us in a graph).  Heads
+ * of their own over 16-position blocks: the same and the issue of instructions (24 sequences of 5 drafted positions, 8 heads of 64: 65 us;
  * 0.46 instructions a cycle and scheduler, 23 % of DRAM).
- * Measured against, on the same cases: the first launch's two passes over the choice with one barrier a count, or with every key ranked
- * against every other (a 4,096-block choice: 12 to 20 thousand cycles, now 6.7); scores written to the peers one by one (262,144
- * positions 22 us); 2 x 64 positions a tile at head_dim 256, one thread block an SM (49 us); means four lanes each instead of eight
- * (46 us); the tiles of the always attended blocks not asked for early (182 us on the 256 rows). */
+ * Measured against, on the same cases: a choice that counts by barriers, or ranks every key against every other (among 4,096 blocks 12 to
+ * 20 thousand cycles, now 7); scores written to the peers one by one (262,144 positions 22 us); 2 x 64 positions a tile at head_dim 256, one thread block an SM (49 us); means four lanes each instead of eight
+ * (46 us); the tiles of the always attended blocks not asked for early (7 us more on the 256 rows). */
 #include "../../include/silvann_b200.h"
 #include "common.cuh"
 #include "kernels.h"
@@ -50,7 +49,7 @@ static constexpr int SPARSE_DEVICES = 64;
 #define SP_THREADS (SP_WARPS * 32)
 #define SP_CHUNK 4096u                        /* scores looked at in one go; the best of the chunks before them ride along */
 #define SP_CAP (SP_CHUNK + SILVANN_B200_PAGED_KEEP_MAX + 8u)
-#define SP_LIST 512u                          /* candidates among which the border is looked for: sixteen a lane */
+#define SP_LIST 512u                          /* scores among which a warp looks for the border: sixteen a lane */
 
 template <int D> struct SparseCfg {
     static constexpr int TP = D == 256 ? 32 : D == 128 ? 64 : 128;         /* positions a tile: 32 KB of K and V */
@@ -79,12 +78,14 @@ struct SparseParams {
     uint64_t q_stride;
     PagedDiv per;                       /* blocks a page */
     uint32_t seqs, stride, pool_pages, page_pos, block, q_heads, kv_heads, group, head_blocks, first, last, top;
-    uint32_t block_log, table_blocks, chunk, cap, choice_top, ring_bytes, choice_at, free_stages;      /* scores looked at in one go, and room for them; the ring, or what lies in its place before, at its end */
+    uint32_t block_log, table_blocks;   /* blocks that a table row has columns for */
+    uint32_t chunk, cap, choice_top;    /* scores looked at in one go, room for them, room for the chosen */
+    uint32_t ring_bytes, choice_at, free_stages;      /* the ring, or what lies in its place before; where that begins; stages ahead of it */
     float scale_log2;
     bool o_wide;                        /* o starts on 8 bytes */
 };
 
-/* 16-bit values as doubles without a conversion (those run at a quarter of the multiply-adds' rate): the exponent and
+/* 16-bit values as doubles without a conversion (a shift and a mask run beside the multiply-adds, conversions take longer than them): the exponent and
  * mantissa bits moved to their place in a double's high word, which is the value times 2^-896 (bf16) or 2^-1008 (fp16),
  * subnormals included.  The query sum carries 2^800 or 2^900, so a score comes out times 2^-SHIFT.  An infinity
  * or a NaN would come out finite: `special` collects the magnitudes, and a mean that has one is summed again by conversion. */
@@ -150,7 +151,7 @@ __device__ __forceinline__ void hist_walk(const Choice S, uint32_t need, int lan
     }
 }
 
-/* Where many scores are equal, or many blocks are chosen: the `take`-th greatest key found a byte at a time, then two passes
+/* Where the floats do not tell, as among many equal scores: the `take`-th greatest key found a byte at a time, then two passes
  * over all keys, one that counts and one that writes, in index order. */
 __device__ __noinline__ void choose_by_bytes(const Choice S, uint32_t m, uint32_t take) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -439,13 +440,13 @@ paged_sparse_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         return at;
     };
     uint4 x[Cfg::U][Cfg::CPL];
-    auto load = [&](int32_t mine, int g) {                /* rounds g to g + 3 */
+    auto load = [&](int32_t mine, int g) {                /* rounds g to g + 3; from L2: a mean is read once, and may be the grid ahead's work */
 #pragma unroll
         for (int u = g; u < g + 4; ++u) {
             const int32_t at = __shfl_sync(0xffffffffu, mine, u * Cfg::BPS + lane / Cfg::LPB);
             const uint4* src = reinterpret_cast<const uint4*>(P.means + ((size_t)max(at, 0) * P.kv_heads + kvh) * D) + lane % Cfg::LPB;
 #pragma unroll
-            for (int y = 0; y < Cfg::CPL; ++y) x[u][y] = at >= 0 ? __ldg(src + y * Cfg::LPB) : make_uint4(0u, 0u, 0u, 0u);
+            for (int y = 0; y < Cfg::CPL; ++y) x[u][y] = at >= 0 ? __ldcg(src + y * Cfg::LPB) : make_uint4(0u, 0u, 0u, 0u);
         }
     };
     int32_t mine = -1, next = -1;

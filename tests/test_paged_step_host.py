@@ -48,7 +48,8 @@ def test_write_refuses(change):
     {"o": None}, {"q": None}, {"k_pool": None}, {"v_pool": None}, {"k_means": None}, {"row_seq": None}, {"row_pos": None}, {"page_table": None}, {"dtype": -1}, {"head_dim": 96},
     {"head_dim": 512}, {"kv_heads": 0}, {"q_heads": 0}, {"q_heads": 15}, {"q_heads": 130}, {"rows": 0}, {"seqs": 0}, {"table_stride": 0}, {"pool_pages": 0}, {"pool_pages": 1 << 26},
     {"block_positions": 0}, {"block_positions": 48}, {"block_positions": 128}, {"last": 0}, {"first": 1000, "top": 23}, {"top": 0xFFFFFFFF}, {"first": 0xFFFFFFFF, "top": 0xFFFFFFFF},
-    {"q_stride": 16 * 128 - 8}, {"q_stride": 16 * 128 + 4}, {"q": A + 8}, {"k_pool": A + 8}, {"v_pool": A + 2}, {"k_means": A + 8}, {"res": A + 2}, {"page_table": A + 1}])
+    {"q_stride": 16 * 128 - 8}, {"q_stride": 16 * 128 + 4}, {"q": A + 8}, {"k_pool": A + 8}, {"v_pool": A + 2}, {"k_means": A + 8}, {"res": A + 2}, {"page_table": A + 1},
+    {"o": A + 1}, {"rows": (1 << 23) + 1}, {"kv_heads": 8192, "q_heads": 8192}, {"chosen": A + 2}, {"row_pos": A + 1}])
 def test_sparse_refuses(change):
     assert "paged_sparse" in refused(ext.paged_sparse, SPARSE, **change)
 
