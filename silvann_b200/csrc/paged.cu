@@ -113,7 +113,7 @@ __device__ __forceinline__ bool tables_rows(const TablesParams& P, const uint32_
  * memory: the step is decided (it fits or is refused) before anything is written, without an exchange.  Then three flat lists — pages
  * that come back, pages handed out, new positions — are walked by all threads of the cluster.  One barrier of the cluster stands between
  * what reads the caller's arrays and what may write them in place, and between the pages that come back and those handed out.
- * What bounds it: latency.  A step is a handful of dependent reads and searches long (one new position each of 32 sequences: 2.9 us in a
+ * What bounds it: latency.  A step is a handful of dependent reads and searches long (one new position each of 32 sequences: 2.8 us in a
  * graph; of 4,097, some ending: 9.4 us); the cluster is there for the steps that bring many positions (98 thousand from 61 prompts:
  * 11.2 us, 81 us on one thread block). */
 __global__ void __launch_bounds__(SV_TABLES_THREADS, 1) paged_tables_kernel(const TablesParams P) {

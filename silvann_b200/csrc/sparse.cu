@@ -21,8 +21,8 @@
  * What bounds it.  Many rows of moderate length: memory (256 rows of 1,000 to 16,000 positions, 32 heads on 4 of 128, 16 blocks of 128
  * each: 172 us, 6.1 TB/s of means, keys and values).  Long rows: the phases' own chains of trips to memory and through shared
  * memory, during which little is in flight (32 rows of 1,024 to 100,000 positions, 16 heads on 2 of 256: 44 us, of which the tiles
- * are half; 24 us at memory's rate).  One row: that chain alone (8,192 positions 10.4 us, 262,144 positions 19.1 us in a graph).  Heads
- * of their own over 16-position blocks: the same and the issue of instructions (24 sequences of 5 drafted positions, 8 heads of 64: 65 us;
+ * are half; 24 us at memory's rate).  One row: that chain alone (8,192 positions 10.6 us, 262,144 positions 19.6 us in a graph).  Heads
+ * of their own over 16-position blocks: the same and the issue of instructions (24 sequences of 5 drafted positions, 8 heads of 64: 64 us;
  * 0.46 instructions a cycle and scheduler, 23 % of DRAM).
  * Measured against, on the same cases: a choice that counts by barriers, or ranks every key against every other (among 4,096 blocks 12 to
  * 20 thousand cycles, now 7); scores written to the peers one by one (262,144 positions 22 us); 2 x 64 positions a tile at head_dim 256, one thread block an SM (49 us); means four lanes each instead of eight
@@ -246,10 +246,8 @@ __device__ __noinline__ bool choose_few(const Choice S, uint32_t m, uint32_t tak
  * border lies in, which rarely holds more than a few (a tail of scores is thin); one warp finds the border among those. */
 __device__ __noinline__ bool choose_many(const Choice S, uint32_t m, uint32_t take) {
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    /* a thread's scores are neighbours, so that its chosen ones are in order */
-    const uint32_t run = (m + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u) * 4u, i0 = tid * run, i1 = min(m, i0 + run);
     float mn = INFINITY, mx = -INFINITY;
-    for (uint32_t i = i0; i < i1; i += 4u) {                              /* (behind the last there are NaNs up to a multiple of four) */
+    for (uint32_t i = 4u * tid; i < m; i += 4u * SP_THREADS) {             /* (behind the last there are NaNs up to a multiple of four) */
         const float4 y = *reinterpret_cast<const float4*>(S.score() + i);
         const float f[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -265,7 +263,7 @@ __device__ __noinline__ bool choose_many(const Choice S, uint32_t m, uint32_t ta
     for (int w = 0; w < SP_WARPS; ++w) { mn = fminf(mn, __uint_as_float(S.t->warp_in[w])); mx = fmaxf(mx, __uint_as_float(S.t->warp_tie[w])); }
     const float per = mx > mn ? __fdividef(255.99f, mx - mn) : 0.f, low = mx >= mn ? mn : 0.f;
     auto bin_of = [&](float f) { return (uint32_t)min(max((int)((f - low) * per), 0), 255); };     /* does not fall as f rises */
-    for (uint32_t i = i0; i < i1; i += 4u) {
+    for (uint32_t i = 4u * tid; i < m; i += 4u * SP_THREADS) {
         const float4 y = *reinterpret_cast<const float4*>(S.score() + i);
         const float f[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -278,7 +276,7 @@ __device__ __noinline__ bool choose_many(const Choice S, uint32_t m, uint32_t ta
     if (in_bin > SP_LIST) return false;
     float least = -INFINITY;                      /* of the border's step, what reaches this is chosen */
     if (in_bin != need) {
-        for (uint32_t i = i0; i < i1; i += 4u) {
+        for (uint32_t i = 4u * tid; i < m; i += 4u * SP_THREADS) {
             const float4 y = *reinterpret_cast<const float4*>(S.score() + i);
             const float f[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -293,6 +291,8 @@ __device__ __noinline__ bool choose_many(const Choice S, uint32_t m, uint32_t ta
         least = S.t->least;
         if (!(least == least)) return false;
     }
+    /* a thread's scores are neighbours now, so that its chosen ones are in order */
+    const uint32_t run = (m + SP_THREADS * 4u - 1u) / (SP_THREADS * 4u) * 4u, i0 = tid * run, i1 = min(m, i0 + run);
     uint32_t hits = 0u;
     for (uint32_t i = i0, b = 0u; i < i1; i += 4u, b += 4u) {
         const float4 y = *reinterpret_cast<const float4*>(S.score() + i);
