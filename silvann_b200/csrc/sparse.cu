@@ -23,7 +23,7 @@
  * memory, during which little is in flight (32 rows of 1,024 to 100,000 positions, 16 heads on 2 of 256: 44 us, of which the tiles
  * are half; 24 us at memory's rate).  One row: that chain alone (8,192 positions 10.6 us, 262,144 positions 19.6 us in a graph).  Heads
  * of their own over 16-position blocks: the same and the issue of instructions (24 sequences of 5 drafted positions, 8 heads of 64: 64 us;
- * 0.46 instructions a cycle and scheduler, 23 % of DRAM).
+ * 0.48 instructions a cycle and scheduler, 24 % of DRAM).
  * Measured against, on the same cases: a choice that counts by barriers, or ranks every key against every other (among 4,096 blocks 12 to
  * 20 thousand cycles, now 7); scores written to the peers one by one (262,144 positions 22 us); 2 x 64 positions a tile at head_dim 256, one thread block an SM (49 us); means four lanes each instead of eight
  * (46 us); the tiles of the always attended blocks not asked for early (7 us more on the 256 rows). */
@@ -873,7 +873,9 @@ static cudaError_t sparse_launch_one(const CUtensorMap& km, const CUtensorMap& v
     P.free_stages = P.choice_at / Cfg::STAGE_BYTES;
     const size_t smem = rest + P.ring_bytes + (size_t)keep * 4;
     constexpr size_t most = rest + (ring > choice_most ? ring : choice_most) + 127 + SILVANN_B200_PAGED_KEEP_MAX * 4;
-    /* As many thread blocks a row as fit the card at once, as far as a row's longest list of tiles goes round. */
+    /* As many thread blocks a row as fit the card at once, as far as a row's longest list of tiles goes round.  With 1, 2, 4, 8, 16 of them:
+     * 32 long rows of 2 kv heads 115, 71, 44, 56, 94 us (the rule takes 4); one row of 262,144 positions 95, 56, 34, 24, 20 (16); 120 rows of
+     * 8 kv heads 64, 85, 140, 274, 619 (1). */
     const uint32_t fit = (uint32_t)(228 * 1024 / (smem + 1024)), slots = device_sm_count() * (fit < (uint32_t)Cfg::OCC ? fit : (uint32_t)Cfg::OCC);
     const uint32_t tiles = (keep * P.block + Cfg::TP - 1u) / Cfg::TP;
     uint32_t cluster = 1u;
