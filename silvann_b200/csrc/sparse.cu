@@ -59,7 +59,7 @@ template <int D> struct SparseCfg {
     static constexpr int K_BYTES = BOXES * BOX_BYTES;
     static constexpr int STAGE_BYTES = 2 * K_BYTES;       /* K then V */
     static constexpr int STAGES = D == 64 ? 2 : 3;        /* 96 KB, two thread blocks an SM; at 64 64 KB, three */
-    static constexpr int OCC = D == 64 ? 3 : 2;
+    static constexpr int OCC = D == 64 ? 3 : 2;           /* (at 64, on 120 rows of 8 kv heads: 64 us; two an SM 68, four with a ring of one stage 72) */
     /* scores: lanes a mean, 16-byte pieces of it a lane, means a warp takes in a round, rounds asked for at once */
     static constexpr int LPB = D == 256 ? 16 : 8;
     static constexpr int CPL = D / 8 / LPB;
