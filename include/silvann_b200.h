@@ -417,7 +417,7 @@ int silvann_b200_paged_tables(int32_t* new_lens, int32_t* page_table, int32_t* r
  * k_means[slot / B][kv_heads][head_dim]: the fp32 sum of the block's B rows, sixteen in ascending order and those sums in
  * ascending order, over B, rounded to `dtype`.
  * Rows of one block must stand in ascending order next to each other (as paged_tables numbers them), earlier ones in the
- * pool; no slot may be named twice.  kv_heads * head_dim and the strides are multiples of 8, addresses of 16 bytes. */
+ * pool; no slot may be named twice, and the rows may not lie in the pools.  kv_heads * head_dim and the strides are multiples of 8, addresses of 16 bytes. */
 int silvann_b200_paged_write(void* k_pool, void* v_pool, void* k_means, const void* k_rows, const void* v_rows, uint64_t k_stride,
                              uint64_t v_stride, const int32_t* row_slot, uint32_t rows, uint32_t kv_heads, uint32_t head_dim,
                              uint64_t pool_pages, uint32_t page_positions, uint32_t block_positions, int dtype, void* stream);
@@ -436,7 +436,7 @@ int silvann_b200_paged_write(void* k_pool, void* v_pool, void* k_means, const vo
  * negative is padding: its outputs stay as they were; one with row_seq >= seqs is treated the same and raises
  * SILVANN_B200_STATUS_BAD_PAGE.  A row at a negative position attends nothing: o is 0, res (-inf, 0, 0), chosen -1.
  * head_dim 64, 128 or 256; up to 64 query heads a kv head; B 16, 32, 64 or 128 and a divisor of page_positions;
- * first + last + top <= SILVANN_B200_PAGED_KEEP_MAX; rows * kv_heads <= 2^24; rows of q multiples of 8 elements, addresses of q,
+ * first + last + top <= SILVANN_B200_PAGED_KEEP_MAX; rows * kv_heads <= 2^24; no output may overlap an input (q included); rows of q multiples of 8 elements, addresses of q,
  * pools and means of 16 bytes. */
 #define SILVANN_B200_PAGED_KEEP_MAX 1024u
 int silvann_b200_paged_sparse(void* o, float* res, int32_t* chosen, const void* q, uint64_t q_stride, const void* k_pool, const void* v_pool,
